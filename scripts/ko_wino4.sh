@@ -5,7 +5,7 @@ set -e
 cd "$(dirname "$0")/.."
 PKG=disentangled-person-image-generation_amd
 cp $PKG/libdpig_hip.so /tmp/libdpig_hip.so.keep
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -I include -I $PKG/csrc -DDPIG_WINO4_KNOCKOUT -c $PKG/csrc/dpig_conv_wino4.hip -o /tmp/wino4_ko.o
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -fPIC -I include -I $PKG/csrc -DDPIG_WINO4_KNOCKOUT -c $PKG/csrc/dpig_conv_wino4.hip -o /tmp/wino4_ko.o
 objs=$(ls build/obj/*.o | grep -v dpig_conv_wino4.o)
 hipcc --offload-arch=gfx950 -shared -fPIC -o $PKG/libdpig_hip.so $objs /tmp/wino4_ko.o
 for ko in ${KOS:-0 1 2 4 3 7 8}; do

@@ -9,7 +9,7 @@
 set -e
 cd "$(dirname "$0")"
 R=../..; P=$R/disentangled-person-image-generation_amd
-hipcc --offload-arch=gfx950 -O3 -w -o mfma_peak mfma_peak.hip
-hipcc --offload-arch=gfx950 -O3 -w -o hwid_probe hwid_probe.hip
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -w -I $R/include -I $P/csrc -o bhq32_probe bhq32_probe.hip
-hipcc --offload-arch=gfx950 -O3 -std=c++17 -shared -fPIC -DDPIG_TRACE -I $R/include -I $P/csrc -o libdpig_trace.so $P/csrc/*.hip
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -w -o mfma_peak mfma_peak.hip
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -w -o hwid_probe hwid_probe.hip
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -w -I $R/include -I $P/csrc -o bhq32_probe bhq32_probe.hip
+hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -std=c++17 -shared -fPIC -DDPIG_TRACE -I $R/include -I $P/csrc -o libdpig_trace.so $P/csrc/*.hip
