@@ -177,6 +177,20 @@ SYMBOLS = {
     "dpig_act_bwd_pool2x": (_i, [_vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _f, _i, _vp]),
     "dpig_pose_stem_fwd": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _f, _vp, _i, _vp]),
     "dpig_pose_stem_wgrad": (_i, [_vp, _i, _i, _i, _vp, _vp, _i, _i, _i, _vp, _i, _vp]),
+    "dpig_act8_store": (_i, [_vp, _i, _i64, _i64, _i, _i, _vp, _vp, _vp]),
+    "dpig_act8_load": (_i, [_vp, _vp, _i64, _i, _i, _vp, _i, _i64, _vp]),
+    "dpig_act8_act_bwd": (_i, [_vp, _i, _i64, _vp, _i64, _i, _i, _i, _f, _vp, _i64, _vp]),
+    "dpig_rownorm_fwd": (_i, [_vp, _i, _i64, _i64, _i, _i, _vp, _vp, _f, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp]),
+    "dpig_rownorm_bwd_workspace_bytes": (_sz, [_i64, _i]),
+    "dpig_rownorm_bwd": (_i, [_vp, _i, _i64, _vp, _i64, _i, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _sz,
+                              _vp]),
+    "dpig_gated_residual_fwd": (_i, [_vp, _i64, _vp, _i64, _i, _i64, _i, _i, _vp, _vp, _f, _vp, _i, _i64, _vp, _vp, _i64, _vp, _vp, _i, _vp, _vp,
+                                     _i, _vp, _vp, _f, _vp, _i64, _vp, _vp, _i, _vp, _vp, _vp]),
+    "dpig_gated_residual_bwd_workspace_bytes": (_sz, [_i64, _i, _i64]),
+    "dpig_gated_residual_bwd": (_i, [_vp, _i, _i64, _vp, _i64, _i, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _i, _i64, _vp, _vp, _vp, _vp, _i64,
+                                     _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "dpig_linear_wgrad8_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i]),
+    "dpig_linear_wgrad8": (_i, [_vp, _vp, _i, _i64, _i, _vp, _i, _i64, _i, _vp, _vp, _vp, _f, _vp, _f, _vp, _sz, _vp]),
     "dpig_sce_mean": (_i, [_vp, _i, _f, _vp, _vp, _f, _vp]),
     "dpig_logit_mean": (_i, [_vp, _i, _i, _f, _vp, _vp, _f, _vp]),
     "dpig_l1_workspace_bytes": (_sz, [_i64]),

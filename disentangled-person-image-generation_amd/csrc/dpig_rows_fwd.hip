@@ -1,0 +1,267 @@
+// Norms over the channels of a row, at a residual block's entry and at its exit, forward:
+//   entry  y   = scale * xh + offset,            xh = (x - mean) rstd   (kind 'rms': mean = 0)
+//   exit   out = x + res_scale * gate * (scale * fh + offset),  fh the normed f; optionally the next block's entry norm of `out` (as stored) too
+// and, on request, xh (or fh, or the next norm's xh) as an 8-bit checkpoint from the same registers.
+//
+// Bound by HBM: every operand is read once and every result written once, one wave (or less, or a workgroup) per row with the row in
+// registers; a lane asks for the next row before it works on the present one.  A workgroup takes a contiguous range of rows, so the
+// per-channel operands stay in registers and a gate row is loaded when its group begins.
+#include "dpig_rows.h"
+
+namespace dpig {
+namespace rows {
+
+struct EntryP {
+    const void* x; void* y;
+    const float *scale, *offset;
+    float *mean, *rstd;
+    long ldx, ldy, nrows, chunk;
+    int C, layer;
+    float eps, rC;
+    Save save;
+};
+
+template <typename T, int LPR, int NV, bool RAG, bool SAVE>
+__global__ __launch_bounds__(NT) void entry_fwd_kernel(const EntryP p) {
+    constexpr int RPB = NT / LPR;
+    __shared__ float red[1][4];
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const T* x = static_cast<const T*>(p.x);
+    T* y = static_cast<T*>(p.y);
+    int n[NV];
+    float sc[NV][8], of[NV][8];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = 8 * (lane + LPR * j);
+        n[j] = p.C - c;
+        ldp(p.scale, c, p.C, 1.f, sc[j]);
+        ldp(p.offset, c, p.C, 0.f, of[j]);
+    }
+    const long r0 = blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.nrows);
+    long r = r0 + sub;
+    Raw8<T> nx[NV];
+    auto fetch = [&](long row) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j]);
+    };
+    if (r < r1) fetch(r);
+    for (; r < r1; r += RPB) {
+        float v[NV][8];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) unpack(nx[j], v[j]);
+        if (r + RPB < r1) fetch(r + RPB);
+        float mean, rstd;
+        whiten<LPR, NV, RAG>(v, n, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
+        if (lane == 0) {
+            if (p.mean != nullptr) p.mean[r] = mean;
+            p.rstd[r] = rstd;
+        }
+        if (SAVE) save8<LPR, NV>(p.save, r, lane, v);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], sc[j][e], of[j][e]);
+            st8<RAG>(y + r * p.ldy + 8 * (lane + LPR * j), v[j], n[j]);
+        }
+    }
+}
+
+struct ExitP {
+    const void *x, *f;
+    void *out, *h;                       // h == nullptr: no next norm
+    const float *scale, *offset, *res, *scale2, *offset2;
+    const void* gate;
+    float *mean, *rstd, *mean2, *rstd2;
+    long ldx, ldf, ldo, ldh, nrows, chunk, per;      // per = rows of a gate group
+    int C, layer, layer2, gate_bf16;
+    float eps, eps2, rC;
+    Save save, save2;
+};
+
+template <typename T, int LPR, int NV, bool RAG, bool NEXT>
+__global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
+    constexpr int RPB = NT / LPR;
+    __shared__ float red[1][4];
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const T *x = static_cast<const T*>(p.x), *f = static_cast<const T*>(p.f);
+    int n[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) n[j] = p.C - 8 * (lane + LPR * j);
+    const long r0 = blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.nrows);
+    long r = r0 + sub;
+    Raw8<T> nx[NV], nf[NV];
+    auto fetch = [&](long row) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j]);
+            nf[j] = ld8<RAG>(f + row * p.ldf + 8 * (lane + LPR * j), n[j]);
+        }
+    };
+    if (r < r1) fetch(r);
+    long until = r;                      // the rows before it share the gate row that is loaded
+    float a[NV][8], b[NV][8];            // out = x + a fh + b
+    for (; r < r1; r += RPB) {
+        float v[NV][8], xv[NV][8];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) { unpack(nf[j], v[j]); unpack(nx[j], xv[j]); }
+        if (r + RPB < r1) fetch(r + RPB);
+        if (r >= until) {
+            const long g = p.gate != nullptr ? r / p.per : 0;
+            until = p.gate != nullptr ? (g + 1) * p.per : p.nrows;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = 8 * (lane + LPR * j);
+                float m[8], t[8];
+                ldp(p.res, c, p.C, 1.f, m);
+                if (p.gate != nullptr) {
+                    if (p.gate_bf16) ldp(static_cast<const bf16_t*>(p.gate) + g * p.C, c, p.C, 1.f, t);
+                    else ldp(static_cast<const float*>(p.gate) + g * p.C, c, p.C, 1.f, t);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) m[e] *= t[e];
+                }
+                ldp(p.scale, c, p.C, 1.f, a[j]);
+                ldp(p.offset, c, p.C, 0.f, b[j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { a[j][e] *= m[e]; b[j][e] *= m[e]; }
+            }
+        }
+        float mean, rstd;
+        whiten<LPR, NV, RAG>(v, n, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
+        if (lane == 0) {
+            if (p.mean != nullptr) p.mean[r] = mean;
+            p.rstd[r] = rstd;
+        }
+        if (p.save.codes != nullptr) save8<LPR, NV>(p.save, r, lane, v);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] = xv[j][e] + fmaf(v[j][e], a[j][e], b[j][e]);
+            st8<RAG>(static_cast<T*>(p.out) + r * p.ldo + 8 * (lane + LPR * j), v[j], n[j]);
+        }
+        if (NEXT) {
+            // the next block's norm sees `out` as it is stored, so that its backward pass can start from the stored tensor
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool in = RAG ? e < n[j] : n[j] > 0;
+                    v[j][e] = in ? round_to(v[j][e], static_cast<T*>(nullptr)) : 0.f;
+                }
+            whiten<LPR, NV, RAG>(v, n, p.rC, p.layer2 != 0, p.eps2, red, &mean, &rstd);
+            if (lane == 0) {
+                if (p.mean2 != nullptr) p.mean2[r] = mean;
+                p.rstd2[r] = rstd;
+            }
+            if (p.save2.codes != nullptr) save8<LPR, NV>(p.save2, r, lane, v);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = 8 * (lane + LPR * j);
+                float sc[8], of[8];
+                ldp(p.scale2, c, p.C, 1.f, sc);
+                ldp(p.offset2, c, p.C, 0.f, of);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], sc[e], of[e]);
+                st8<RAG>(static_cast<T*>(p.h) + r * p.ldh + c, v[j], n[j]);
+            }
+        }
+    }
+}
+
+// rows per workgroup: a multiple of the rows it takes at a time, about eight workgroups per CU when there are enough rows
+static long fwd_chunk(int64_t nrows, int C) {
+    const long rpb = NT / lanes_per_row(C);
+    const long want = 8L * kNumCU;
+    long it = (nrows + rpb * want - 1) / (rpb * want);
+    return (it < 1 ? 1 : it) * rpb;
+}
+
+static int check_rows(const char* who, int64_t nrows, int C, int kind) {
+    if (nrows <= 0 || nrows > (1L << 40)) return fail(DPIG_EINVAL, "%s: bad row count", who);
+    if (C <= 0 || C > C_MAX) return fail(DPIG_EINVAL, "%s: channels must be 1 .. %d", who, C_MAX);
+    if (kind != DPIG_NORM_LAYER && kind != DPIG_NORM_RMS) return fail(DPIG_EINVAL, "%s: unknown kind of norm", who);
+    return DPIG_OK;
+}
+static int check_save(const char* who, int fmt, const uint8_t* codes, const uint8_t* scales) {
+    if (!codes && !scales) return DPIG_OK;
+    if (!codes || !scales) return fail(DPIG_EINVAL, "%s: a checkpoint needs codes and scales", who);
+    if (fmt != DPIG_ACT8_E4M3 && fmt != DPIG_ACT8_INT8) return fail(DPIG_EINVAL, "%s: unknown checkpoint format", who);
+    if (!aligned16(codes)) return fail(DPIG_EALIGN, "%s: checkpoint codes must be 16-byte aligned", who);
+    return DPIG_OK;
+}
+
+template <typename T> static int entry_fwd(EntryP p, hipStream_t st) {
+    const bool rag = p.C % 8 != 0 || !vec_ok(p.x, p.ldx, sizeof(T)) || !vec_ok(p.y, p.ldy, sizeof(T));
+    const bool save = p.save.codes != nullptr;
+    const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
+#define CALL_RS(L, N, R, S) hipLaunchKernelGGL((entry_fwd_kernel<T, L, N, R, S>), grid, dim3(NT), 0, st, p)
+#define CALL(L, N)                                                                                                         \
+    do {                                                                                                                  \
+        if (rag) { if (save) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
+        else { if (save) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
+    } while (0)
+    DPIG_ROWS_DISPATCH(p.C, CALL);
+#undef CALL
+#undef CALL_RS
+    return check_launch("rownorm_fwd");
+}
+template <typename T> static int exit_fwd(ExitP p, hipStream_t st) {
+    const int z = sizeof(T);
+    const bool rag = p.C % 8 != 0 || !vec_ok(p.x, p.ldx, z) || !vec_ok(p.f, p.ldf, z) || !vec_ok(p.out, p.ldo, z) ||
+                     (p.h != nullptr && !vec_ok(p.h, p.ldh, z));
+    const bool next = p.h != nullptr;
+    const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
+#define CALL_RS(L, N, R, S) hipLaunchKernelGGL((exit_fwd_kernel<T, L, N, R, S>), grid, dim3(NT), 0, st, p)
+#define CALL(L, N)                                                                                                         \
+    do {                                                                                                                  \
+        if (rag) { if (next) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
+        else { if (next) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
+    } while (0)
+    DPIG_ROWS_DISPATCH(p.C, CALL);
+#undef CALL
+#undef CALL_RS
+    return check_launch("gated_residual_fwd");
+}
+
+}  // namespace rows
+}  // namespace dpig
+
+using namespace dpig;
+
+extern "C" int dpig_rownorm_fwd(const void* x, int is_bf16, int64_t ldx, int64_t nrows, int C, int kind, const float* scale, const float* offset,
+                                float eps, void* y, int64_t ldy, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales,
+                                void* stream) {
+    if (int rc = rows::check_rows("rownorm_fwd", nrows, C, kind)) return rc;
+    if (int rc = rows::check_save("rownorm_fwd", fmt, codes, scales)) return rc;
+    if (!x || !y || !rstd || (kind == DPIG_NORM_LAYER && !mean)) return fail(DPIG_EINVAL, "rownorm_fwd: null pointer");
+    if (ldx < C || ldy < C) return fail(DPIG_EINVAL, "rownorm_fwd: row stride below the channel count");
+    rows::EntryP p = {x, y, scale, offset, kind == DPIG_NORM_LAYER ? mean : nullptr, rstd, (long)ldx, (long)ldy, (long)nrows,
+                      rows::fwd_chunk(nrows, C), C, kind == DPIG_NORM_LAYER, eps, 1.0f / (float)C, {codes, scales, fmt, act8::padded(C)}};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return is_bf16 ? rows::entry_fwd<rows::bf16_t>(p, st) : rows::entry_fwd<float>(p, st);
+}
+
+extern "C" int dpig_gated_residual_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, int is_bf16, int64_t nrows, int C, int kind,
+                                       const float* scale, const float* offset, float eps, const void* gate, int gate_bf16, int64_t groups,
+                                       const float* res_scale, void* out, int64_t ldo, float* mean, float* rstd, int fmt, uint8_t* codes,
+                                       uint8_t* scales, int kind2, const float* scale2, const float* offset2, float eps2, void* h,
+                                       int64_t ldh, float* mean2, float* rstd2, int fmt2, uint8_t* codes2, uint8_t* scales2,
+                                       void* stream) {
+    if (int rc = rows::check_rows("gated_residual_fwd", nrows, C, kind)) return rc;
+    if (int rc = rows::check_save("gated_residual_fwd", fmt, codes, scales)) return rc;
+    if (!x || !f || !out || !rstd || (kind == DPIG_NORM_LAYER && !mean)) return fail(DPIG_EINVAL, "gated_residual_fwd: null pointer");
+    if (ldx < C || ldf < C || ldo < C || (h && ldh < C)) return fail(DPIG_EINVAL, "gated_residual_fwd: row stride below the channel count");
+    if (gate && (groups <= 0 || nrows % groups != 0)) return fail(DPIG_EINVAL, "gated_residual_fwd: rows must be a multiple of the gate's groups");
+    if (h) {
+        if (int rc = rows::check_rows("gated_residual_fwd (next norm)", nrows, C, kind2)) return rc;
+        if (int rc = rows::check_save("gated_residual_fwd (next norm)", fmt2, codes2, scales2)) return rc;
+        if (!rstd2 || (kind2 == DPIG_NORM_LAYER && !mean2)) return fail(DPIG_EINVAL, "gated_residual_fwd: null pointer (next norm)");
+    }
+    const int ld8 = act8::padded(C);
+    rows::ExitP p = {x, f, out, h, scale, offset, res_scale, scale2, offset2, gate, kind == DPIG_NORM_LAYER ? mean : nullptr, rstd,
+                     kind2 == DPIG_NORM_LAYER ? mean2 : nullptr, rstd2, (long)ldx, (long)ldf, (long)ldo, (long)ldh, (long)nrows,
+                     rows::fwd_chunk(nrows, C), gate ? (long)(nrows / groups) : (long)nrows, C, kind == DPIG_NORM_LAYER,
+                     kind2 == DPIG_NORM_LAYER, gate_bf16, eps, eps2, 1.0f / (float)C, {codes, scales, fmt, ld8},
+                     {h ? codes2 : nullptr, scales2, fmt2, ld8}};
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return is_bf16 ? rows::exit_fwd<rows::bf16_t>(p, st) : rows::exit_fwd<float>(p, st);
+}

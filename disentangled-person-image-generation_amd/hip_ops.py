@@ -1403,6 +1403,335 @@ def linear_wgrad(x, dy, out=None, beta=0.0):
     return out
 
 
+# ---- residual blocks on rows of channels: 8-bit activation checkpoints, entry norm, gated exit (csrc/dpig_act8.hip, dpig_rows_*.hip, dpig_wgrad8.hip) ----
+# Rows are every leading axis, channels the last one; fp32 or bf16 tensors, fp32 parameters.  Scratch comes from torch's allocator call by call, so
+# that calls on different streams and captured graphs never share it.
+ACT8_FORMATS = {"e4m3": 0, "int8": 1}
+NORM_KINDS = {"layer": 0, "rms": 1}
+
+
+class Act8(object):
+    """An activation checkpoint in 8 bits: `codes` [rows, ld] uint8 (ld = channels rounded up to 32), `scales` [rows, ld / 32] uint8 (the
+    power of two 2^(byte - 127) that 32 channels share; 255: the group held a value that was not finite and comes back as NaN), the
+    `shape` of the tensor it stands for, and `fmt` 'e4m3' (8-bit floats: relative precision 2^-4) or 'int8' (integers plus 128: 1/64 to 1/127 of the
+    group's largest value).  A value that is not zero keeps its sign.  33/32 bytes an element."""
+    __slots__ = ("codes", "scales", "shape", "fmt")
+
+    def __init__(self, codes, scales, shape, fmt):
+        shape = tuple(int(n) for n in shape)
+        _fmt8(fmt)
+        if not shape or shape[-1] < 1:
+            raise RuntimeError("Act8: the last axis (channels) must not be empty, got shape %s" % (shape,))
+        rows, ld = _prod(shape[:-1]), -(-shape[-1] // 32) * 32
+        for t, want in ((codes, (rows, ld)), (scales, (rows, ld // 32))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous():
+                raise RuntimeError("Act8: need contiguous uint8 %s, got %s %s" % (want, t.dtype, tuple(t.shape)))
+        if codes.device != scales.device:
+            raise RuntimeError("Act8: codes on %s, scales on %s" % (codes.device, scales.device))
+        self.codes, self.scales, self.shape, self.fmt = codes, scales, shape, fmt
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+
+def _prod(dims):
+    n = 1
+    for d in dims:
+        n *= d
+    return n
+
+
+def _fmt8(fmt):
+    try:
+        return ACT8_FORMATS[fmt]
+    except (KeyError, TypeError):
+        raise RuntimeError("8-bit format must be one of %s, got %r" % (sorted(ACT8_FORMATS), fmt))
+
+
+def _kind(kind):
+    try:
+        return NORM_KINDS[kind]
+    except (KeyError, TypeError):
+        raise RuntimeError("norm kind must be one of %s, got %r" % (sorted(NORM_KINDS), kind))
+
+
+def _rows_of(t, what="tensor", like=None):
+    """(tensor, rows, C, ld) of an fp32 / bf16 tensor as rows of channels; copied only if its rows are not evenly spaced runs of channels.
+    `like`: a tensor whose shape, type and device it has to share."""
+    _require_dev(t)
+    if like is None:
+        if t.device.index != torch.cuda.current_device():
+            raise RuntimeError("%s is on %s but the current device is cuda:%d (kernels run on its current stream)"
+                               % (what, t.device, torch.cuda.current_device()))
+    elif t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+        raise RuntimeError("%s is %s %s on %s, expected %s %s on %s" % (what, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype,
+                                                                       like.device))
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise RuntimeError("%s has no channels (shape %s)" % (what, tuple(t.shape)))
+    C = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // C, C, C
+    if t.dim() == 2 and (t.stride(1) == 1 or C == 1) and t.stride(0) >= C:
+        return t, t.shape[0], C, t.stride(0)
+    if t.dim() == 4 and t.numel():
+        ld = nhwc_ld(t)
+        if ld is not None:
+            return t, t.numel() // C, C, ld
+    t = t.contiguous()
+    return t, t.numel() // C, C, C
+
+
+def _chan(t, C, what, device):
+    """Per-channel fp32 parameter [C] (None passes)."""
+    if t is None:
+        return None
+    if t.dtype != F32 or t.numel() != C or t.device != device:
+        raise RuntimeError("%s must be %d fp32 values on %s, got %s %s on %s" % (what, C, device, tuple(t.shape), t.dtype, t.device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _row_stat(t, rows, what, device):
+    if t is None:
+        return None
+    if t.dtype != F32 or t.numel() != rows or t.device != device:
+        raise RuntimeError("%s must be %d fp32 values on %s, got %s %s on %s" % (what, rows, device, tuple(t.shape), t.dtype, t.device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _new_act8(shape, rows, C, fmt, device):
+    ld = -(-C // 32) * 32
+    return Act8(torch.empty((rows, ld), dtype=torch.uint8, device=device), torch.empty((rows, ld // 32), dtype=torch.uint8, device=device), shape, fmt)
+
+
+def _scratch(nbytes, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def act8_store(x, fmt="e4m3"):
+    """x (fp32 or bf16, channels on the last axis) -> its 8-bit checkpoint."""
+    f = _fmt8(fmt)
+    x, rows, C, ld = _rows_of(x, "x")
+    a = _new_act8(x.shape, rows, C, fmt, x.device)
+    if rows:
+        check(lib().dpig_act8_store(ptr(x), int(x.dtype == BF16), ld, rows, C, f, ptr(a.codes), ptr(a.scales), stream_ptr()), "act8_store")
+    return a
+
+
+def _act8_on(a, device):
+    if a.codes.device != device:
+        raise RuntimeError("the checkpoint is on %s, expected %s" % (a.codes.device, device))
+
+
+def _current_device():
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def act8_load(a, dtype=F32):
+    """The values a checkpoint stands for, as fp32 or (exactly) bf16."""
+    if dtype not in (F32, BF16):
+        raise RuntimeError("act8_load: fp32 or bf16, got %s" % dtype)
+    if not a.codes.is_cuda:
+        raise RuntimeError("dpig HIP ops need device tensors (got %s): there is no CPU fallback" % a.codes.device)
+    _act8_on(a, _current_device())
+    y = torch.empty(a.shape, dtype=dtype, device=a.codes.device)
+    rows, C = a.codes.shape[0], a.shape[-1]
+    if rows:
+        check(lib().dpig_act8_load(ptr(a.codes), ptr(a.scales), rows, C, _fmt8(a.fmt), ptr(y), int(dtype == BF16), C, stream_ptr()), "act8_load")
+    return y
+
+
+def act8_act_bwd(dy, a, act, alpha=0.2):
+    """dz = dy * act'(y), y the ReLU / LeakyReLU output that the checkpoint `a` holds (its codes keep y's sign)."""
+    if act not in (ACT_RELU, ACT_LRELU):
+        raise RuntimeError("act8_act_bwd: the activation must be ReLU or LeakyReLU")
+    dy, rows, C, ld = _rows_of(dy, "dy")
+    if tuple(dy.shape) != a.shape:
+        raise RuntimeError("act8_act_bwd: dy is %s, the checkpoint stands for %s" % (tuple(dy.shape), a.shape))
+    _act8_on(a, dy.device)
+    dz = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    if rows:
+        check(lib().dpig_act8_act_bwd(ptr(dy), int(dy.dtype == BF16), ld, ptr(a.codes), rows, C, _fmt8(a.fmt), act, alpha, ptr(dz), C,
+                                      stream_ptr()), "act8_act_bwd")
+    return dz
+
+
+def linear_wgrad8(a, dy, scale=None, offset=None, out=None, beta=0.0, want_bias=False, db=None, db_beta=0.0):
+    """dw[C, K] = beta * dw + x^T @ dy with x = scale * (the checkpoint's values) + offset, in fp32; `want_bias`: (dw, db) with the column sums
+    db[K] = db_beta * db + sum dy.  dy fp32 or bf16, rows as the checkpoint's.  `out` / `db`: contiguous fp32 buffers to write or add into."""
+    dy, rows, K, ld = _rows_of(dy, "dy")
+    C = a.shape[-1]
+    if rows != a.codes.shape[0]:
+        raise RuntimeError("linear_wgrad8: dy has %d rows, the checkpoint %d" % (rows, a.codes.shape[0]))
+    _act8_on(a, dy.device)
+    scale, offset = _chan(scale, C, "scale", dy.device), _chan(offset, C, "offset", dy.device)
+    for t, n, what in ((out, C * K, "out"), (db, K, "db")):
+        if t is not None and (t.dtype != F32 or t.numel() != n or not t.is_contiguous() or t.device != dy.device):
+            raise RuntimeError("linear_wgrad8: %s must be %d contiguous fp32 values on %s" % (what, n, dy.device))
+    if out is None:
+        out, beta = torch.empty((C, K), dtype=F32, device=dy.device), 0.0
+    want_bias = want_bias or db is not None
+    if want_bias and db is None:
+        db, db_beta = torch.empty(K, dtype=F32, device=dy.device), 0.0
+    if rows == 0:
+        for t, b in ((out, beta), (db, db_beta)):
+            if t is not None:
+                t.mul_(b) if b else t.zero_()
+        return (out, db) if want_bias else out
+    bf = int(dy.dtype == BF16)
+    affine = int(scale is not None or offset is not None)
+    nbytes = lib().dpig_linear_wgrad8_workspace_bytes(rows, C, K, bf, affine)
+    ws = _scratch(nbytes, dy.device)
+    check(lib().dpig_linear_wgrad8(ptr(a.codes), ptr(a.scales), _fmt8(a.fmt), rows, C, ptr(dy), bf, ld, K, ptr(scale), ptr(offset), ptr(out),
+                                   float(beta), ptr(db), float(db_beta), ptr(ws), nbytes, stream_ptr()), "linear_wgrad8")
+    return (out, db) if want_bias else out
+
+
+def rownorm_fwd(x, scale=None, offset=None, eps=1e-5, kind="layer", save8=None):
+    """(y, mean, rstd, saved): y = scale * xh + offset over the last axis, xh = (x - mean) * rstd ('rms': mean is None and not subtracted).
+    `save8` ('e4m3' | 'int8'): `saved` is xh as an 8-bit checkpoint, written in the same pass; else None."""
+    k = _kind(kind)
+    f = _fmt8(save8) if save8 is not None else 0
+    x, rows, C, ld = _rows_of(x, "x")
+    dev = x.device
+    scale, offset = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean = torch.empty(rows, dtype=F32, device=dev) if k == 0 else None
+    rstd = torch.empty(rows, dtype=F32, device=dev)
+    a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
+    if rows:
+        check(lib().dpig_rownorm_fwd(ptr(x), int(x.dtype == BF16), ld, rows, C, k, ptr(scale), ptr(offset), eps, ptr(y), C, ptr(mean), ptr(rstd),
+                                     f, ptr(a.codes) if a else None, ptr(a.scales) if a else None, stream_ptr()), "rownorm_fwd")
+    return y, mean, rstd, a
+
+
+def _saved_operand(saved, like, rows):
+    """(x pointer, ld, fmt, codes pointer, scales pointer, keep-alive) of a norm's saved input: the tensor itself or the checkpoint of its normed
+    values."""
+    if isinstance(saved, Act8):
+        if saved.shape != tuple(like.shape):
+            raise RuntimeError("the checkpoint stands for %s, the gradient is %s" % (saved.shape, tuple(like.shape)))
+        _act8_on(saved, like.device)
+        return None, 0, _fmt8(saved.fmt), ptr(saved.codes), ptr(saved.scales), saved
+    t, _, _, ld = _rows_of(saved, "saved", like)
+    return ptr(t), ld, 0, None, None, t
+
+
+def rownorm_bwd(dy, saved, scale, mean, rstd, kind="layer", accum=None, want_params=True):
+    """(dx, dscale, doffset) of rownorm_fwd; `saved` is its input x or the checkpoint of xh, `accum` (as dy) is added to dx.  The parameter gradients
+    are None with want_params=False."""
+    k = _kind(kind)
+    dy, rows, C, ld = _rows_of(dy, "dy")
+    dev = dy.device
+    scale = _chan(scale, C, "scale", dev)
+    xp, ldx, f, codes, scales, keep = _saved_operand(saved, dy, rows)
+    mean, rstd = _row_stat(mean, rows, "mean", dev), _row_stat(rstd, rows, "rstd", dev)
+    if rstd is None or (k == 0 and mean is None and xp is not None):
+        raise RuntimeError("rownorm_bwd: the statistics of the forward pass are needed")
+    lda = 0
+    if accum is not None:
+        accum, _, _, lda = _rows_of(accum, "accum", dy)
+    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+    dscale = torch.empty(C, dtype=F32, device=dev) if want_params else None
+    doffset = torch.empty(C, dtype=F32, device=dev) if want_params else None
+    if rows == 0:
+        if want_params:
+            dscale.zero_(), doffset.zero_()
+        return dx, dscale, doffset
+    nbytes = lib().dpig_rownorm_bwd_workspace_bytes(rows, C) if want_params else 0
+    ws = _scratch(nbytes, dev)
+    check(lib().dpig_rownorm_bwd(ptr(dy), int(dy.dtype == BF16), ld, xp, ldx, f, codes, scales, rows, C, k, ptr(scale), ptr(mean), ptr(rstd),
+                                 ptr(accum), lda, ptr(dx), C, ptr(dscale), ptr(doffset), ptr(ws), nbytes, stream_ptr()), "rownorm_bwd")
+    return dx, dscale, doffset
+
+
+def _gate_groups(gate, x, rows, C):
+    """(contiguous gate, groups): the gate's leading axes have to be the first ones of x (trailing ones of length 1 are dropped), or, for
+    rows x [R, C], any divisor of R."""
+    if gate is None:
+        return None, 0
+    if gate.dtype not in (F32, BF16) or gate.device != x.device or gate.dim() == 0 or gate.shape[-1] != C:
+        raise RuntimeError("gate must be fp32 or bf16 [..., %d] on %s, got %s %s on %s" % (C, x.device, tuple(gate.shape), gate.dtype, gate.device))
+    lead = list(gate.shape[:-1])
+    while lead and lead[-1] == 1:
+        lead.pop()
+    ok = lead == list(x.shape[:-1])[:len(lead)] or (len(lead) == 1 and x.dim() == 2 and lead[0] > 0 and rows % lead[0] == 0)
+    if not ok:
+        raise RuntimeError("gate is %s, which is neither a prefix of the rows of x %s nor a divisor of them" % (tuple(gate.shape), tuple(x.shape)))
+    return gate.contiguous(), _prod(lead)
+
+
+def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None, eps=1e-5, kind="layer", save8=None, next_norm=None, next_save8=None):
+    """The exit of a residual block: out = x + res_scale * gate * (scale * fh + offset), fh the normed f.  -> (out, mean, rstd, saved, after).
+    gate: [C], [G, C] for groups of consecutive rows (a gate per sample), or as x.  `save8`: `saved` is fh as a checkpoint.
+    `next_norm` = (scale, offset, eps, kind): also the entry norm of the next block on `out`, in the same pass -- `after` is what rownorm_fwd(out, ...,
+    save8=next_save8) returns; else None."""
+    k = _kind(kind)
+    q = _fmt8(save8) if save8 is not None else 0
+    x, rows, C, ldx = _rows_of(x, "x")
+    f, _, _, ldf = _rows_of(f, "f", x)
+    dev = x.device
+    scale, offset, res_scale = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev), _chan(res_scale, C, "res_scale", dev)
+    gate, groups = _gate_groups(gate, x, rows, C)
+    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean = torch.empty(rows, dtype=F32, device=dev) if k == 0 else None
+    rstd = torch.empty(rows, dtype=F32, device=dev)
+    a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
+    h = mean2 = rstd2 = a2 = scale2 = offset2 = None
+    k2, q2, eps2 = 0, 0, 0.0
+    if next_norm is not None:
+        scale2, offset2, eps2, kind2 = next_norm
+        k2 = _kind(kind2)
+        q2 = _fmt8(next_save8) if next_save8 is not None else 0
+        scale2, offset2 = _chan(scale2, C, "the next norm's scale", dev), _chan(offset2, C, "the next norm's offset", dev)
+        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        mean2 = torch.empty(rows, dtype=F32, device=dev) if k2 == 0 else None
+        rstd2 = torch.empty(rows, dtype=F32, device=dev)
+        a2 = _new_act8(x.shape, rows, C, next_save8, dev) if next_save8 is not None else None
+    elif next_save8 is not None:
+        raise RuntimeError("gated_residual_fwd: next_save8 without next_norm")
+    if rows:
+        check(lib().dpig_gated_residual_fwd(
+            ptr(x), ldx, ptr(f), ldf, int(x.dtype == BF16), rows, C, k, ptr(scale), ptr(offset), eps, ptr(gate),
+            int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(out), C, ptr(mean), ptr(rstd), q, ptr(a.codes) if a else None,
+            ptr(a.scales) if a else None, k2, ptr(scale2), ptr(offset2), eps2, ptr(h), C, ptr(mean2), ptr(rstd2), q2,
+            ptr(a2.codes) if a2 else None, ptr(a2.scales) if a2 else None, stream_ptr()), "gated_residual_fwd")
+    return out, mean, rstd, a, ((h, mean2, rstd2, a2) if next_norm is not None else None)
+
+
+def gated_residual_bwd(dout, saved, scale, offset, gate, res_scale, mean, rstd, kind="layer", want_params=True):
+    """(df, dscale, doffset, dgate, dres_scale) of gated_residual_fwd without its next norm; the gradient of x is dout itself.  `saved` is f or the
+    checkpoint of fh.  dgate (in gate's shape and type) and dres_scale are None where the forward pass had none; with want_params=False all but df."""
+    k = _kind(kind)
+    dout, rows, C, ld = _rows_of(dout, "dout")
+    dev = dout.device
+    scale, offset, res_scale = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev), _chan(res_scale, C, "res_scale", dev)
+    gate, groups = _gate_groups(gate, dout, rows, C)
+    fp, ldf, q, codes, scales, keep = _saved_operand(saved, dout, rows)
+    mean, rstd = _row_stat(mean, rows, "mean", dev), _row_stat(rstd, rows, "rstd", dev)
+    if rstd is None or (k == 0 and mean is None and fp is not None):
+        raise RuntimeError("gated_residual_bwd: the statistics of the forward pass are needed")
+    df = torch.empty(dout.shape, dtype=dout.dtype, device=dev)
+    dscale = doffset = dgate = dres = None
+    if want_params:
+        dscale = torch.empty(C, dtype=F32, device=dev)
+        doffset = torch.empty(C, dtype=F32, device=dev)
+        dgate = torch.empty_like(gate) if gate is not None else None
+        dres = torch.empty(C, dtype=F32, device=dev) if res_scale is not None else None
+    if rows == 0:
+        for t in (dscale, doffset, dgate, dres):
+            if t is not None:
+                t.zero_()
+        return df, dscale, doffset, dgate, dres
+    nbytes = lib().dpig_gated_residual_bwd_workspace_bytes(rows, C, groups) if want_params else 0
+    ws = _scratch(nbytes, dev)
+    check(lib().dpig_gated_residual_bwd(
+        ptr(dout), int(dout.dtype == BF16), ld, fp, ldf, q, codes, scales, rows, C, k, ptr(scale), ptr(offset), ptr(gate),
+        int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(mean), ptr(rstd), ptr(df), C, ptr(dscale), ptr(doffset), ptr(dgate),
+        ptr(dres), ptr(ws), nbytes, stream_ptr()), "gated_residual_bwd")
+    return df, dscale, doffset, dgate, dres
+
+
 def crop_resize_fwd(img, boxes, box_ind, ch, cw):
     _require_dev(img)
     img = img.contiguous()

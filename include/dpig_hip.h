@@ -616,6 +616,65 @@ int dpig_axpby3d(const float* src, int64_t s_outer, int64_t s_row, float* dst, i
  * physically NHWC activation, and its gradient. */
 int dpig_transpose12(const void* x, void* y, int B, int A, int C, int elem_bytes, void* stream);
 
+/* ---- residual blocks on rows of channels: entry norm, gated exit, 8-bit activation checkpoints --------------------
+ * Beyond the reference's graph (its residual blocks, models.py:398-400 / 474-515, have neither norm nor gate): the same blocks with a norm over
+ * the channels before and after, a gate and a residual scale, and activations kept for the backward pass in 8 bits.
+ * Rows are every leading axis ([rows][C], a row stride ld* in elements, any alignment the element type allows); fp32 or bf16 tensors (is_bf16), fp32
+ * parameters [C]; statistics and sums in fp32.  C is 1 .. 8192 where a norm is taken. */
+#define DPIG_NORM_LAYER 0       /* xh = (x - mean) rstd                                                                  */
+#define DPIG_NORM_RMS 1         /* xh = x rstd, rstd = 1 / sqrt(mean_c x^2 + eps); mean pointers may be NULL               */
+
+/* A checkpoint: codes [rows][ld8], ld8 = C rounded up to 32, 16-byte aligned, and scales [rows][ld8 / 32], the byte e + 127 of the power of two
+ * that 32 channels share, the smallest with max|x| <= 448 * 2^e / 127 * 2^e (e in -116 .. 119 / 121).  Codes are x / 2^e rounded to nearest even as
+ * OCP e4m3 floats or as integers plus 128; a value that is not zero keeps its sign (at least the smallest code).  A group that holds a
+ * value that is not finite has scale byte 255 and zero codes and comes back as NaN.  Code * 2^e is exact in bf16. */
+#define DPIG_ACT8_E4M3 0
+#define DPIG_ACT8_INT8 1
+int dpig_act8_store(const void* x, int is_bf16, int64_t ldx, int64_t rows, int C, int fmt, uint8_t* codes, uint8_t* scales,
+                    void* stream);
+int dpig_act8_load(const uint8_t* codes, const uint8_t* scales, int64_t rows, int C, int fmt, void* y, int is_bf16, int64_t ldy,
+                   void* stream);
+/* dz = dy * act'(y) with the sign of y read from its checkpoint (ReLU, LeakyReLU). */
+int dpig_act8_act_bwd(const void* dy, int is_bf16, int64_t lddy, const uint8_t* codes, int64_t rows, int C, int fmt, int act, float alpha,
+                      void* dz, int64_t lddz, void* stream);
+
+/* y = scale * xh + offset (scale / offset NULL: 1 / 0); mean, rstd [rows]; codes / scales (or both NULL): xh as a checkpoint. */
+int dpig_rownorm_fwd(const void* x, int is_bf16, int64_t ldx, int64_t rows, int C, int kind, const float* scale, const float* offset,
+                     float eps, void* y, int64_t ldy, float* mean, float* rstd, int fmt, uint8_t* codes, uint8_t* scales,
+                     void* stream);
+/* dx = gradient of the above (+ accum, may be NULL), from x and its statistics or (x NULL) from the checkpoint of xh; dscale / doffset may be NULL.
+ * The workspace is needed for the parameter gradients only. */
+size_t dpig_rownorm_bwd_workspace_bytes(int64_t rows, int C);
+int dpig_rownorm_bwd(const void* dy, int is_bf16, int64_t lddy, const void* x, int64_t ldx, int fmt, const uint8_t* codes,
+                     const uint8_t* scales, int64_t rows, int C, int kind, const float* scale, const float* mean, const float* rstd,
+                     const void* accum, int64_t ldacc, void* dx, int64_t lddx, float* dscale, float* doffset, void* ws,
+                     size_t ws_bytes, void* stream);
+
+/* out = x + res_scale * gate * (scale * fh + offset), fh the normed f.  gate [groups][C] (fp32, or bf16 with gate_bf16; NULL: 1) serves
+ * rows / groups consecutive rows each; res_scale [C] (NULL: 1).  codes / scales (or both NULL): fh as a checkpoint.
+ * h not NULL: also h = scale2 * oh + offset2 with oh the normed `out` as stored -- the next block's entry -- and its checkpoint codes2 / scales2. */
+int dpig_gated_residual_fwd(const void* x, int64_t ldx, const void* f, int64_t ldf, int is_bf16, int64_t rows, int C, int kind,
+                            const float* scale, const float* offset, float eps, const void* gate, int gate_bf16, int64_t groups,
+                            const float* res_scale, void* out, int64_t ldo, float* mean, float* rstd, int fmt, uint8_t* codes,
+                            uint8_t* scales, int kind2, const float* scale2, const float* offset2, float eps2, void* h, int64_t ldh,
+                            float* mean2, float* rstd2, int fmt2, uint8_t* codes2, uint8_t* scales2, void* stream);
+/* Gradients of the above without h (dx is dout itself): df, and dscale / doffset / dgate (as gate) / dres_scale, each may be NULL.
+ * groups of the workspace query: 0 without a gate. */
+size_t dpig_gated_residual_bwd_workspace_bytes(int64_t rows, int C, int64_t groups);
+int dpig_gated_residual_bwd(const void* dout, int is_bf16, int64_t lddo, const void* f, int64_t ldf, int fmt, const uint8_t* codes,
+                            const uint8_t* scales, int64_t rows, int C, int kind, const float* scale, const float* offset,
+                            const void* gate, int gate_bf16, int64_t groups, const float* res_scale, const float* mean,
+                            const float* rstd, void* df, int64_t lddf, float* dscale, float* doffset, void* dgate,
+                            float* dres_scale, void* ws, size_t ws_bytes, void* stream);
+
+/* Filter gradient from a checkpoint: dw[C][K] = beta * dw + sum_r (scale * q + offset)[r][c] * dy[r][k] (scale / offset [C], NULL: 1 / 0), and
+ * db[K] = beta_b * db + sum_r dy (NULL: not wanted).  The result is that of fp32 products and sums for fp32 and bf16 dy alike.
+ * `affine` of the query: scale or offset is given. */
+size_t dpig_linear_wgrad8_workspace_bytes(int64_t rows, int C, int K, int dy_bf16, int affine);
+int dpig_linear_wgrad8(const uint8_t* codes, const uint8_t* scales, int fmt, int64_t rows, int C, const void* dy, int dy_bf16, int64_t lddy,
+                       int K, const float* scale, const float* offset, float* dw, float beta, float* db, float beta_b, void* ws,
+                       size_t ws_bytes, void* stream);
+
 /* ---- losses (trainer.py:238-245, 607, 623) --------------------------------------------------- */
 /* out[0] = mean_i sce(logits_i, label) ; dlogits_i = scale*(sigmoid(x_i)-label)/n (dlogits may be NULL) */
 int dpig_sce_mean(const float* logits, int n, float label, float* out, float* dlogits, float scale,
