@@ -189,7 +189,7 @@ SYMBOLS = {
     "dpig_gated_residual_bwd_workspace_bytes": (_sz, [_i64, _i, _i64]),
     "dpig_gated_residual_bwd": (_i, [_vp, _i, _i64, _vp, _i64, _i, _vp, _vp, _i64, _i, _i, _vp, _vp, _vp, _i, _i64, _vp, _vp, _vp, _vp, _i64,
                                      _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "dpig_linear_wgrad8_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i]),
+    "dpig_linear_wgrad8_workspace_bytes": (_sz, [_i64, _i, _i64, _i, _i, _i]),
     "dpig_linear_wgrad8": (_i, [_vp, _vp, _i, _i64, _i, _vp, _i, _i64, _i, _vp, _vp, _vp, _f, _vp, _f, _vp, _sz, _vp]),
     "dpig_sce_mean": (_i, [_vp, _i, _f, _vp, _vp, _f, _vp]),
     "dpig_logit_mean": (_i, [_vp, _i, _i, _f, _vp, _vp, _f, _vp]),
@@ -230,6 +230,11 @@ def ptr(t):
 
 def stream_ptr():
     return torch.cuda.current_stream().cuda_stream
+
+
+def raw_stream(device_index):
+    """torch's current stream on a device as the C ABI takes it, without building a Stream object (0.1 us instead of 2.8 us)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 class _Workspace:

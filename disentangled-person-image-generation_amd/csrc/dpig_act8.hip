@@ -27,7 +27,7 @@ template <typename T, bool RAG, int F>
 __global__ __launch_bounds__(NT) void store_kernel(const P p) {
     ACT8_FOR(r, v) {
         float x[8];
-        unpack(ld8<RAG>(static_cast<const T*>(p.x) + r * p.ldx + 8 * v, p.C - 8 * v), x);
+        unpack(ld8<RAG>(static_cast<const T*>(p.x) + r * p.ldx + 8 * v, p.C - 8 * v, false), x);
         save8_as<F>(x, p.codes + r * p.ld8 + 8 * v, p.scales + r * (p.ld8 >> 5) + (v >> 2), (v & 3) == 0);
     }
 }
@@ -43,11 +43,12 @@ __global__ __launch_bounds__(NT) void load_kernel(const P p) {
 }
 template <typename T, bool RAG, int F>
 __global__ __launch_bounds__(NT) void mask_kernel(const P p) {
+    const long safe = safe_rows(p.nrows, p.C);
     const float off = p.act == DPIG_ACT_RELU ? 0.f : p.alpha;
     ACT8_FOR(r, v) {
         const uint2 q = *reinterpret_cast<const uint2*>(p.codes + r * p.ld8 + 8 * v);
         float d[8];
-        unpack(ld8<RAG>(static_cast<const T*>(p.x) + r * p.ldx + 8 * v, p.C - 8 * v), d);
+        unpack(ld8<RAG>(static_cast<const T*>(p.x) + r * p.ldx + 8 * v, p.C - 8 * v, r < safe), d);
 #pragma unroll
         for (int e = 0; e < 8; ++e) d[e] *= act8::positive<F>(e < 4 ? q.x : q.y, e & 3) ? 1.f : off;
         st8<RAG>(static_cast<T*>(p.y) + r * p.ldy + 8 * v, d, p.C - 8 * v);

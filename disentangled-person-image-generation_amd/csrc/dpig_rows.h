@@ -42,12 +42,16 @@ __device__ __forceinline__ void pack(const float (&v)[8], Raw8<bf16_t>& r) {
     r.a.z = (unsigned)f2bf(v[4]) | ((unsigned)f2bf(v[5]) << 16); r.a.w = (unsigned)f2bf(v[6]) | ((unsigned)f2bf(v[7]) << 16);
 }
 
-// n (<= 0: none, >= 8: all) elements at p; the others are zero
-template <bool RAG, typename T> __device__ __forceinline__ Raw8<T> ld8(const T* p, int n) {
+// n (<= 0: none, >= 8: all) elements at p.  RAG: what lies behind the n is not to be used -- `beyond` says that 8 elements may be read at p
+// all the same, which holds for every row but the last where C >= 8 (see `safe_rows`), so that only the last row's partial vector is read
+// element by element.
+// Rows whose partial vector may be read whole: its 8 elements end before column C + 7 <= ld + C, the end of the next row, if there is one.
+__device__ __forceinline__ long safe_rows(long nrows, int C) { return C >= 8 ? nrows - 1 : 0; }
+template <bool RAG, typename T> __device__ __forceinline__ Raw8<T> ld8(const T* p, int n, bool beyond) {
     Raw8<T> r = {};
     if (!RAG) {
         if (n > 0) r = *reinterpret_cast<const Raw8<T>*>(p);
-    } else if (n >= 8) {
+    } else if (n >= 8 || (n > 0 && beyond)) {
         __builtin_memcpy(&r, p, sizeof(r));
     } else if (n > 0) {
         T t[8];
@@ -64,12 +68,15 @@ template <bool RAG, typename T> __device__ __forceinline__ void st8(T* p, const 
         if (n > 0) *reinterpret_cast<Raw8<T>*>(p) = r;
     } else if (n >= 8) {
         __builtin_memcpy(p, &r, sizeof(r));
-    } else if (n > 0) {
+    } else if (n > 0) {                                  // 4 + 2 + 1 elements
         T t[8];
         __builtin_memcpy(t, &r, sizeof(r));
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < n) p[e] = t[e];
+        if (n & 4) __builtin_memcpy(p, t, 4 * sizeof(T));
+        if (n & 2) {
+            const T u[2] = {n & 4 ? t[4] : t[0], n & 4 ? t[5] : t[1]};
+            __builtin_memcpy(p + (n & 4), u, 2 * sizeof(T));
+        }
+        if (n & 1) p[n & 6] = n & 4 ? (n & 2 ? t[6] : t[4]) : (n & 2 ? t[2] : t[0]);
     }
 }
 // per-channel fp32 parameters (any 4-byte alignment); `def` where there is no tensor or no channel
@@ -117,10 +124,23 @@ template <int LPR, int NS> __device__ __forceinline__ void row_sums(float (&s)[N
     }
 }
 
+// s / C and 1 / sqrt(a), each within about half a step: the scale of a whole row hangs on them, and with it the side on which every value of the
+// row falls when it is rounded to 8 bits
+__device__ __forceinline__ float over_count(float s, float C, float rC) {
+    const float q = s * rC;
+    return fmaf(fmaf(-q, C, s), rC, q);
+}
+__device__ __forceinline__ float inv_sqrt(float a) {
+    const float r = __builtin_amdgcn_rsqf(a);
+    const float h = a * r, l = fmaf(a, r, -h);
+    const float e = fmaf(-l, r, fmaf(-h, r, 1.f));           // 1 - a r r
+    return fmaf(0.5f * r, e, r);
+}
+
 // Statistics of a row held in registers, and the row normed in place: mean first, then the sum of squares about it (no cancellation).
-// n[j] <= 0: a vector outside the row; a partial vector's tail is kept zero.
+// n[j] <= 0: a vector outside the row (zero); what is behind a partial vector's end is ignored and comes out as zero.
 template <int LPR, int NV, bool RAG>
-__device__ __forceinline__ void whiten(float (&v)[NV][8], const int (&n)[NV], float rC, bool layer, float eps, float (*red)[4], float* mean,
+__device__ __forceinline__ void whiten(float (&v)[NV][8], const int (&n)[NV], float C, float rC, bool layer, float eps, float (*red)[4], float* mean,
                                        float* rstd) {
     float s[1];
     float mu = 0.f;
@@ -129,9 +149,9 @@ __device__ __forceinline__ void whiten(float (&v)[NV][8], const int (&n)[NV], fl
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[0] += v[j][e];
+            for (int e = 0; e < 8; ++e) s[0] += !RAG || e < n[j] ? v[j][e] : 0.f;
         row_sums<LPR, 1>(s, red);
-        mu = s[0] * rC;
+        mu = over_count(s[0], C, rC);
     }
     s[0] = 0.f;
 #pragma unroll
@@ -143,7 +163,7 @@ __device__ __forceinline__ void whiten(float (&v)[NV][8], const int (&n)[NV], fl
             s[0] += v[j][e] * v[j][e];
         }
     row_sums<LPR, 1>(s, red);
-    const float r = rsqrtf(s[0] * rC + eps);
+    const float r = inv_sqrt(over_count(s[0], C, rC) + eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -183,18 +203,31 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
     }
 }
 
-// launch shape of a row length: lanes per row and vectors per lane
+// Launch shape of a row length: lanes per row and vectors per lane, the smallest that holds it.  The steps of three vectors keep at least two lanes
+// of three at work for every length above 64 (640 channels: 80 of 96 lane-vectors; powers of two alone would give 80 of 128, and took 30 us
+// instead of 24 for the exit's gradient of 32768 rows).
 #define DPIG_ROWS_DISPATCH(C, CALL)                      \
     do {                                                 \
         if ((C) <= 64) { CALL(8, 1); }                   \
         else if ((C) <= 128) { CALL(16, 1); }            \
+        else if ((C) <= 192) { CALL(8, 3); }             \
         else if ((C) <= 256) { CALL(32, 1); }            \
+        else if ((C) <= 384) { CALL(16, 3); }            \
         else if ((C) <= 512) { CALL(64, 1); }            \
+        else if ((C) <= 768) { CALL(32, 3); }            \
         else if ((C) <= 1024) { CALL(64, 2); }           \
+        else if ((C) <= 1536) { CALL(64, 3); }           \
         else if ((C) <= 2048) { CALL(256, 1); }          \
+        else if ((C) <= 4096) { CALL(256, 2); }          \
         else { CALL(256, 4); }                           \
     } while (0)
-inline int lanes_per_row(int C) { return C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256; }
+inline int lanes_per_row(int C) {
+    int lanes = 0;
+#define DPIG_ROWS_LANES(L, N) lanes = L
+    DPIG_ROWS_DISPATCH(C, DPIG_ROWS_LANES);
+#undef DPIG_ROWS_LANES
+    return lanes;
+}
 inline bool vec_ok(const void* p, int64_t ld, int esize) { return aligned16(p) && (ld * esize) % 16 == 0; }
 
 }  // namespace rows

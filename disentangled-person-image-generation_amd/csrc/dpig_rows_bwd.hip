@@ -34,6 +34,7 @@ __global__ __launch_bounds__(NT) void rows_bwd_kernel(const BwdP p) {
     constexpr int RPB = NT / LPR;
     __shared__ float red[2][4];
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const long safe = safe_rows(p.nrows, p.C);
     const T *dy = static_cast<const T*>(p.dy), *x = static_cast<const T*>(p.x), *ac = static_cast<const T*>(p.accum);
     int n[NV];
     float w[NV][8], A[NV][8], B[NV][8];
@@ -84,7 +85,7 @@ __global__ __launch_bounds__(NT) void rows_bwd_kernel(const BwdP p) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = 8 * (lane + LPR * j);
-            nd[j] = ld8<RAG>(dy + row * p.lddy + c, n[j]);
+            nd[j] = ld8<RAG>(dy + row * p.lddy + c, n[j], row < safe);
             if (SAVED) {
                 nc.q[j] = make_uint2(0, 0);
                 nc.s[j] = 0;
@@ -93,9 +94,9 @@ __global__ __launch_bounds__(NT) void rows_bwd_kernel(const BwdP p) {
                     nc.s[j] = p.scales[row * (p.ld8 >> 5) + (c >> 5)];
                 }
             } else {
-                nx[j] = ld8<RAG>(x + row * p.ldx + c, n[j]);
+                nx[j] = ld8<RAG>(x + row * p.ldx + c, n[j], row < safe);
             }
-            if (!GROUPS && ac != nullptr) na[j] = ld8<RAG>(ac + row * p.ldacc + c, n[j]);
+            if (!GROUPS && ac != nullptr) na[j] = ld8<RAG>(ac + row * p.ldacc + c, n[j], row < safe);
         }
     };
     float Ag[NV][8], Bg[NV][8];          // groups form: the present group's sums
@@ -106,6 +107,10 @@ __global__ __launch_bounds__(NT) void rows_bwd_kernel(const BwdP p) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 unpack(nd[j], d[j]);
+                if (RAG) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) d[j][e] = e < n[j] ? d[j][e] : 0.f;
+                }
                 if (SAVED) {
                     const float s = act8::scale_value(nc.s[j]);
                     if (p.fmt == DPIG_ACT8_E4M3) act8::decode8<DPIG_ACT8_E4M3>(nc.q[j], s, xh[j]);
@@ -214,7 +219,8 @@ __global__ __launch_bounds__(NT) void rows_bwd_kernel(const BwdP p) {
 }
 
 // ---- the partials' sums ---------------------------------------------------------------------------------------------------------------
-constexpr int FC = 16, FL = 64;          // channels and summing lanes of a workgroup (1024 threads)
+constexpr int FC = 16, FL = 64, FW = FC * FL / 64;          // channels, summing lanes and waves of a workgroup (1024 threads)
+constexpr int FG = 8;                                       // groups that rows_groups_kernel sums at a time
 struct FinP {
     const float* partial;                // [n][2][C]
     float* partial2;                     // [gridDim.y][2][C]: gate-weighted sums over the groups of a workgroup (first launch of two)
@@ -225,19 +231,29 @@ struct FinP {
     long n, ngroups, gpb;                // n: partials per group; gpb: groups of a workgroup
     int C, gate_bf16;
 };
-// sum over the FL lanes of a workgroup, in order; the result in lane 0 of the channel
-__device__ __forceinline__ void fin_sum(float& a, float& b, float (*red)[FL][FC], int cl, int ln) {
-    __syncthreads();
-    red[0][ln][cl] = a;
-    red[1][ln][cl] = b;
-    __syncthreads();
+// sums over the four lanes of a wave that hold one channel; then thread (k, channel) adds the waves' values, always in the same order
+template <int NG> __device__ __forceinline__ void fin_waves(float (&a)[NG], float (&b)[NG], float (*red)[FW][2][FC]) {
 #pragma unroll
-    for (int h = FL / 2; h >= 1; h >>= 1) {
-        if (ln < h) { red[0][ln][cl] += red[0][ln + h][cl]; red[1][ln][cl] += red[1][ln + h][cl]; }
-        __syncthreads();
+    for (int k = 0; k < NG; ++k) {
+        a[k] += __shfl_xor(a[k], 16, 64);
+        b[k] += __shfl_xor(b[k], 16, 64);
+        a[k] += __shfl_xor(a[k], 32, 64);
+        b[k] += __shfl_xor(b[k], 32, 64);
     }
-    a = red[0][0][cl];
-    b = red[1][0][cl];
+    __syncthreads();                     // (red may still be read from the call before)
+    if ((threadIdx.x & 63) < FC) {
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            red[k][threadIdx.x >> 6][0][threadIdx.x & 15] = a[k];
+            red[k][threadIdx.x >> 6][1][threadIdx.x & 15] = b[k];
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void fin_add(const float (*red)[2][FC], int cl, float* a, float* b) {
+    *a = *b = 0.f;
+#pragma unroll
+    for (int w = 0; w < FW; ++w) { *a += red[w][0][cl]; *b += red[w][1][cl]; }
 }
 __device__ __forceinline__ void fin_outputs(const FinP& p, int c, float a, float b) {
     const float rs = p.res ? p.res[c] : 1.f;
@@ -245,9 +261,10 @@ __device__ __forceinline__ void fin_outputs(const FinP& p, int c, float a, float
     if (p.doffset) p.doffset[c] = rs * b;
     if (p.dres) p.dres[c] = (p.scale ? p.scale[c] : 1.f) * a + (p.offset ? p.offset[c] : 0.f) * b;
 }
-// pieces form with a gate: per group the sums over its pieces, dgate, and the gate-weighted sums over the groups of this workgroup
+// pieces form with a gate: per group the sums over its pieces, dgate, and the gate-weighted sums over the groups of this workgroup.
+// FG groups at a time, all their loads in flight together; thread (k, channel) closes group k.
 __global__ __launch_bounds__(FC * FL) void rows_groups_kernel(const FinP p) {
-    __shared__ float red[2][FL][FC];
+    __shared__ float red[FG][FW][2][FC];
     const int cl = threadIdx.x % FC, ln = threadIdx.x / FC, c = blockIdx.x * FC + cl;
     const bool in = c < p.C;
     const float sc = in && p.scale ? p.scale[c] : 1.f, of = in && p.offset ? p.offset[c] : 0.f, rs = in && p.res ? p.res[c] : 1.f;
@@ -268,29 +285,46 @@ __global__ __launch_bounds__(FC * FL) void rows_groups_kernel(const FinP p) {
     if (p.n == 1) {                      // a lane takes whole groups
         for (long g = g0 + ln; g < g1; g += FL)
             if (in) close(g, p.partial[g * 2 * p.C + c], p.partial[(g * 2 + 1) * p.C + c]);
-        fin_sum(wa, wb, red, cl, ln);
     } else {
-        for (long g = g0; g < g1; ++g) {
-            float a = 0.f, b = 0.f;
-            for (long s = ln; s < p.n; s += FL)
-                if (in) { a += p.partial[(g * p.n + s) * 2 * p.C + c]; b += p.partial[((g * p.n + s) * 2 + 1) * p.C + c]; }
-            fin_sum(a, b, red, cl, ln);
-            if (in && ln == 0) close(g, a, b);
+        for (long g = g0; g < g1; g += FG) {
+            float a[FG], b[FG];
+#pragma unroll
+            for (int k = 0; k < FG; ++k) {
+                a[k] = b[k] = 0.f;
+                if (in && g + k < g1)
+                    for (long s = ln; s < p.n; s += FL) {
+                        const float* q = p.partial + ((g + k) * p.n + s) * 2 * p.C + c;
+                        a[k] += q[0];
+                        b[k] += q[p.C];
+                    }
+            }
+            fin_waves<FG>(a, b, red);
+            if (in && ln < FG && g + ln < g1) {
+                float ta, tb;
+                fin_add(red[ln], cl, &ta, &tb);
+                close(g + ln, ta, tb);
+            }
         }
     }
+    float a[1] = {wa}, b[1] = {wb};
+    fin_waves<1>(a, b, red);
     if (!in || ln != 0) return;
+    fin_add(red[0], cl, &wa, &wb);
     if (gridDim.y == 1) { fin_outputs(p, c, wa, wb); return; }
     p.partial2[(long)blockIdx.y * 2 * p.C + c] = wa;
     p.partial2[((long)blockIdx.y * 2 + 1) * p.C + c] = wb;
 }
 __global__ __launch_bounds__(FC * FL) void rows_final_kernel(const FinP p) {
-    __shared__ float red[2][FL][FC];
+    __shared__ float red[1][FW][2][FC];
     const int cl = threadIdx.x % FC, ln = threadIdx.x / FC, c = blockIdx.x * FC + cl;
-    float a = 0.f, b = 0.f;
+    float a[1] = {0.f}, b[1] = {0.f};
     if (c < p.C)
-        for (long s = ln; s < p.n; s += FL) { a += p.partial[s * 2 * p.C + c]; b += p.partial[(s * 2 + 1) * p.C + c]; }
-    fin_sum(a, b, red, cl, ln);
-    if (c < p.C && ln == 0) fin_outputs(p, c, a, b);
+#pragma unroll 4
+        for (long s = ln; s < p.n; s += FL) { a[0] += p.partial[s * 2 * p.C + c]; b[0] += p.partial[(s * 2 + 1) * p.C + c]; }
+    fin_waves<1>(a, b, red);
+    if (c >= p.C || ln != 0) return;
+    fin_add(red[0], cl, a, b);
+    fin_outputs(p, c, a[0], b[0]);
 }
 
 // ---- plan ------------------------------------------------------------------------------------------------------------------------------
@@ -324,7 +358,7 @@ static Plan plan(int64_t nrows, int C, bool gated, int64_t groups) {
     q.chunk = up(sets, pieces) * rpb;
     q.pieces = up(per, q.chunk);
     q.blocks = q.pieces * groups;
-    q.blocks2 = groups < 256 ? groups : 256;
+    q.blocks2 = groups <= 4 * FG ? 1 : (groups / (2 * FG) < 256 ? groups / (2 * FG) : 256);
     return q;
 }
 static size_t ws_bytes(const Plan& q, int C) {

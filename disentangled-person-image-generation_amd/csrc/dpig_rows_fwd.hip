@@ -26,6 +26,7 @@ __global__ __launch_bounds__(NT) void entry_fwd_kernel(const EntryP p) {
     constexpr int RPB = NT / LPR;
     __shared__ float red[1][4];
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const long safe = safe_rows(p.nrows, p.C);
     const T* x = static_cast<const T*>(p.x);
     T* y = static_cast<T*>(p.y);
     int n[NV];
@@ -42,7 +43,7 @@ __global__ __launch_bounds__(NT) void entry_fwd_kernel(const EntryP p) {
     Raw8<T> nx[NV];
     auto fetch = [&](long row) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j]);
+        for (int j = 0; j < NV; ++j) nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j], row < safe);
     };
     if (r < r1) fetch(r);
     for (; r < r1; r += RPB) {
@@ -51,7 +52,7 @@ __global__ __launch_bounds__(NT) void entry_fwd_kernel(const EntryP p) {
         for (int j = 0; j < NV; ++j) unpack(nx[j], v[j]);
         if (r + RPB < r1) fetch(r + RPB);
         float mean, rstd;
-        whiten<LPR, NV, RAG>(v, n, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
+        whiten<LPR, NV, RAG>(v, n, (float)p.C, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
         if (lane == 0) {
             if (p.mean != nullptr) p.mean[r] = mean;
             p.rstd[r] = rstd;
@@ -78,11 +79,13 @@ struct ExitP {
     Save save, save2;
 };
 
-template <typename T, int LPR, int NV, bool RAG, bool NEXT>
+// EACH: every row has a gate of its own, fetched with the row; else a gate row is loaded when its group begins
+template <typename T, int LPR, int NV, bool RAG, bool NEXT, bool EACH>
 __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
     constexpr int RPB = NT / LPR;
     __shared__ float red[1][4];
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const long safe = safe_rows(p.nrows, p.C);
     const T *x = static_cast<const T*>(p.x), *f = static_cast<const T*>(p.f);
     int n[NV];
 #pragma unroll
@@ -90,43 +93,57 @@ __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
     const long r0 = blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.nrows);
     long r = r0 + sub;
     Raw8<T> nx[NV], nf[NV];
+    float ng[NV][8];                     // EACH: the next row's gate
+    auto load_gate = [&](long g, int j, float (&m)[8]) {
+        const int c = 8 * (lane + LPR * j);
+        if (p.gate_bf16) ldp(static_cast<const bf16_t*>(p.gate) + g * p.C, c, p.C, 1.f, m);
+        else ldp(static_cast<const float*>(p.gate) + g * p.C, c, p.C, 1.f, m);
+    };
     auto fetch = [&](long row) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j]);
-            nf[j] = ld8<RAG>(f + row * p.ldf + 8 * (lane + LPR * j), n[j]);
+            const bool beyond = row < safe;
+            nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j], beyond);
+            nf[j] = ld8<RAG>(f + row * p.ldf + 8 * (lane + LPR * j), n[j], beyond);
+            if (EACH) load_gate(row, j, ng[j]);
         }
     };
     if (r < r1) fetch(r);
-    long until = r;                      // the rows before it share the gate row that is loaded
-    float a[NV][8], b[NV][8];            // out = x + a fh + b
+    float a[NV][8], b[NV][8], m[NV][8];  // out = x + m (a fh + b): a, b with the residual scale, m the gate
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const int c = 8 * (lane + LPR * j);
+        float t[8];
+        ldp(p.res, c, p.C, 1.f, t);
+        ldp(p.scale, c, p.C, 1.f, a[j]);
+        ldp(p.offset, c, p.C, 0.f, b[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { a[j][e] *= t[e]; b[j][e] *= t[e]; m[j][e] = 1.f; }
+    }
+    long g = EACH || p.gate == nullptr ? 0 : r / p.per, until = p.gate == nullptr ? p.nrows : (g + 1) * p.per;     // r's group, and its end
+    if (!EACH && p.gate != nullptr && r < r1) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) load_gate(g, j, m[j]);
+    }
     for (; r < r1; r += RPB) {
         float v[NV][8], xv[NV][8];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) { unpack(nf[j], v[j]); unpack(nx[j], xv[j]); }
-        if (r + RPB < r1) fetch(r + RPB);
-        if (r >= until) {
-            const long g = p.gate != nullptr ? r / p.per : 0;
-            until = p.gate != nullptr ? (g + 1) * p.per : p.nrows;
+        for (int j = 0; j < NV; ++j) {
+            unpack(nf[j], v[j]);
+            unpack(nx[j], xv[j]);
+            if (EACH) {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = 8 * (lane + LPR * j);
-                float m[8], t[8];
-                ldp(p.res, c, p.C, 1.f, m);
-                if (p.gate != nullptr) {
-                    if (p.gate_bf16) ldp(static_cast<const bf16_t*>(p.gate) + g * p.C, c, p.C, 1.f, t);
-                    else ldp(static_cast<const float*>(p.gate) + g * p.C, c, p.C, 1.f, t);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) m[e] *= t[e];
-                }
-                ldp(p.scale, c, p.C, 1.f, a[j]);
-                ldp(p.offset, c, p.C, 0.f, b[j]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) { a[j][e] *= m[e]; b[j][e] *= m[e]; }
+                for (int e = 0; e < 8; ++e) m[j][e] = ng[j][e];
             }
         }
+        if (r + RPB < r1) fetch(r + RPB);
+        if (!EACH && r >= until) {
+            while (r >= until) { ++g; until += p.per; }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) load_gate(g, j, m[j]);
+        }
         float mean, rstd;
-        whiten<LPR, NV, RAG>(v, n, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
+        whiten<LPR, NV, RAG>(v, n, (float)p.C, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
         if (lane == 0) {
             if (p.mean != nullptr) p.mean[r] = mean;
             p.rstd[r] = rstd;
@@ -135,7 +152,7 @@ __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = xv[j][e] + fmaf(v[j][e], a[j][e], b[j][e]);
+            for (int e = 0; e < 8; ++e) v[j][e] = fmaf(m[j][e], fmaf(v[j][e], a[j][e], b[j][e]), xv[j][e]);
             st8<RAG>(static_cast<T*>(p.out) + r * p.ldo + 8 * (lane + LPR * j), v[j], n[j]);
         }
         if (NEXT) {
@@ -147,7 +164,7 @@ __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
                     const bool in = RAG ? e < n[j] : n[j] > 0;
                     v[j][e] = in ? round_to(v[j][e], static_cast<T*>(nullptr)) : 0.f;
                 }
-            whiten<LPR, NV, RAG>(v, n, p.rC, p.layer2 != 0, p.eps2, red, &mean, &rstd);
+            whiten<LPR, NV, RAG>(v, n, (float)p.C, p.rC, p.layer2 != 0, p.eps2, red, &mean, &rstd);
             if (lane == 0) {
                 if (p.mean2 != nullptr) p.mean2[r] = mean;
                 p.rstd2[r] = rstd;
@@ -210,7 +227,9 @@ template <typename T> static int exit_fwd(ExitP p, hipStream_t st) {
                      (p.h != nullptr && !vec_ok(p.h, p.ldh, z));
     const bool next = p.h != nullptr;
     const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
-#define CALL_RS(L, N, R, S) hipLaunchKernelGGL((exit_fwd_kernel<T, L, N, R, S>), grid, dim3(NT), 0, st, p)
+    const bool each = p.gate != nullptr && p.per == 1;
+#define CALL_E(L, N, R, S, E) hipLaunchKernelGGL((exit_fwd_kernel<T, L, N, R, S, E>), grid, dim3(NT), 0, st, p)
+#define CALL_RS(L, N, R, S) do { if (each) CALL_E(L, N, R, S, true); else CALL_E(L, N, R, S, false); } while (0)
 #define CALL(L, N)                                                                                                         \
     do {                                                                                                                  \
         if (rag) { if (next) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
@@ -218,6 +237,7 @@ template <typename T> static int exit_fwd(ExitP p, hipStream_t st) {
     } while (0)
     DPIG_ROWS_DISPATCH(p.C, CALL);
 #undef CALL
+#undef CALL_E
 #undef CALL_RS
     return check_launch("gated_residual_fwd");
 }

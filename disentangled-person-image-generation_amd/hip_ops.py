@@ -1456,14 +1456,18 @@ def _kind(kind):
         raise RuntimeError("norm kind must be one of %s, got %r" % (sorted(NORM_KINDS), kind))
 
 
+def _on_current(device, what):
+    if device.index != torch._C._cuda_getDevice():
+        raise RuntimeError("%s is on %s but the current device is cuda:%d (kernels run on its current stream)"
+                           % (what, device, torch.cuda.current_device()))
+
+
 def _rows_of(t, what="tensor", like=None):
     """(tensor, rows, C, ld) of an fp32 / bf16 tensor as rows of channels; copied only if its rows are not evenly spaced runs of channels.
     `like`: a tensor whose shape, type and device it has to share."""
     _require_dev(t)
     if like is None:
-        if t.device.index != torch.cuda.current_device():
-            raise RuntimeError("%s is on %s but the current device is cuda:%d (kernels run on its current stream)"
-                               % (what, t.device, torch.cuda.current_device()))
+        _on_current(t.device, what)
     elif t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
         raise RuntimeError("%s is %s %s on %s, expected %s %s on %s" % (what, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype,
                                                                        like.device))
@@ -1501,20 +1505,30 @@ def _row_stat(t, rows, what, device):
 
 def _new_act8(shape, rows, C, fmt, device):
     ld = -(-C // 32) * 32
-    return Act8(torch.empty((rows, ld), dtype=torch.uint8, device=device), torch.empty((rows, ld // 32), dtype=torch.uint8, device=device), shape, fmt)
+    a = Act8.__new__(Act8)                       # (its own layout: nothing to check)
+    a.codes = torch.empty((rows, ld), dtype=torch.uint8, device=device)
+    a.scales = torch.empty((rows, ld // 32), dtype=torch.uint8, device=device)
+    a.shape, a.fmt = tuple(shape), fmt
+    return a
 
 
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
+def _like_rows(t):
+    """A contiguous tensor of t's shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def act8_store(x, fmt="e4m3"):
     """x (fp32 or bf16, channels on the last axis) -> its 8-bit checkpoint."""
     f = _fmt8(fmt)
     x, rows, C, ld = _rows_of(x, "x")
-    a = _new_act8(x.shape, rows, C, fmt, x.device)
+    dev = x.device
+    a = _new_act8(x.shape, rows, C, fmt, dev)
     if rows:
-        check(lib().dpig_act8_store(ptr(x), int(x.dtype == BF16), ld, rows, C, f, ptr(a.codes), ptr(a.scales), stream_ptr()), "act8_store")
+        check(lib().dpig_act8_store(ptr(x), int(x.dtype == BF16), ld, rows, C, f, ptr(a.codes), ptr(a.scales), _lib.raw_stream(dev.index)), "act8_store")
     return a
 
 
@@ -1523,21 +1537,18 @@ def _act8_on(a, device):
         raise RuntimeError("the checkpoint is on %s, expected %s" % (a.codes.device, device))
 
 
-def _current_device():
-    return torch.device("cuda", torch.cuda.current_device())
-
-
 def act8_load(a, dtype=F32):
     """The values a checkpoint stands for, as fp32 or (exactly) bf16."""
     if dtype not in (F32, BF16):
         raise RuntimeError("act8_load: fp32 or bf16, got %s" % dtype)
+    dev = a.codes.device
     if not a.codes.is_cuda:
-        raise RuntimeError("dpig HIP ops need device tensors (got %s): there is no CPU fallback" % a.codes.device)
-    _act8_on(a, _current_device())
-    y = torch.empty(a.shape, dtype=dtype, device=a.codes.device)
+        raise RuntimeError("dpig HIP ops need device tensors (got %s): there is no CPU fallback" % dev)
+    _on_current(dev, "the checkpoint")
+    y = torch.empty(a.shape, dtype=dtype, device=dev)
     rows, C = a.codes.shape[0], a.shape[-1]
     if rows:
-        check(lib().dpig_act8_load(ptr(a.codes), ptr(a.scales), rows, C, _fmt8(a.fmt), ptr(y), int(dtype == BF16), C, stream_ptr()), "act8_load")
+        check(lib().dpig_act8_load(ptr(a.codes), ptr(a.scales), rows, C, _fmt8(a.fmt), ptr(y), int(dtype == BF16), C, _lib.raw_stream(dev.index)), "act8_load")
     return y
 
 
@@ -1548,11 +1559,12 @@ def act8_act_bwd(dy, a, act, alpha=0.2):
     dy, rows, C, ld = _rows_of(dy, "dy")
     if tuple(dy.shape) != a.shape:
         raise RuntimeError("act8_act_bwd: dy is %s, the checkpoint stands for %s" % (tuple(dy.shape), a.shape))
-    _act8_on(a, dy.device)
-    dz = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    dev = dy.device
+    _act8_on(a, dev)
+    dz = _like_rows(dy)
     if rows:
         check(lib().dpig_act8_act_bwd(ptr(dy), int(dy.dtype == BF16), ld, ptr(a.codes), rows, C, _fmt8(a.fmt), act, alpha, ptr(dz), C,
-                                      stream_ptr()), "act8_act_bwd")
+                                      _lib.raw_stream(dev.index)), "act8_act_bwd")
     return dz
 
 
@@ -1563,8 +1575,9 @@ def linear_wgrad8(a, dy, scale=None, offset=None, out=None, beta=0.0, want_bias=
     C = a.shape[-1]
     if rows != a.codes.shape[0]:
         raise RuntimeError("linear_wgrad8: dy has %d rows, the checkpoint %d" % (rows, a.codes.shape[0]))
-    _act8_on(a, dy.device)
-    scale, offset = _chan(scale, C, "scale", dy.device), _chan(offset, C, "offset", dy.device)
+    dev = dy.device
+    _act8_on(a, dev)
+    scale, offset = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev)
     for t, n, what in ((out, C * K, "out"), (db, K, "db")):
         if t is not None and (t.dtype != F32 or t.numel() != n or not t.is_contiguous() or t.device != dy.device):
             raise RuntimeError("linear_wgrad8: %s must be %d contiguous fp32 values on %s" % (what, n, dy.device))
@@ -1580,10 +1593,10 @@ def linear_wgrad8(a, dy, scale=None, offset=None, out=None, beta=0.0, want_bias=
         return (out, db) if want_bias else out
     bf = int(dy.dtype == BF16)
     affine = int(scale is not None or offset is not None)
-    nbytes = lib().dpig_linear_wgrad8_workspace_bytes(rows, C, K, bf, affine)
-    ws = _scratch(nbytes, dy.device)
+    nbytes = lib().dpig_linear_wgrad8_workspace_bytes(rows, C, ld, K, bf, affine)
+    ws = _scratch(nbytes, dev)
     check(lib().dpig_linear_wgrad8(ptr(a.codes), ptr(a.scales), _fmt8(a.fmt), rows, C, ptr(dy), bf, ld, K, ptr(scale), ptr(offset), ptr(out),
-                                   float(beta), ptr(db), float(db_beta), ptr(ws), nbytes, stream_ptr()), "linear_wgrad8")
+                                   float(beta), ptr(db), float(db_beta), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "linear_wgrad8")
     return (out, db) if want_bias else out
 
 
@@ -1595,13 +1608,13 @@ def rownorm_fwd(x, scale=None, offset=None, eps=1e-5, kind="layer", save8=None):
     x, rows, C, ld = _rows_of(x, "x")
     dev = x.device
     scale, offset = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev)
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    y = _like_rows(x)
     mean = torch.empty(rows, dtype=F32, device=dev) if k == 0 else None
     rstd = torch.empty(rows, dtype=F32, device=dev)
     a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
     if rows:
         check(lib().dpig_rownorm_fwd(ptr(x), int(x.dtype == BF16), ld, rows, C, k, ptr(scale), ptr(offset), eps, ptr(y), C, ptr(mean), ptr(rstd),
-                                     f, ptr(a.codes) if a else None, ptr(a.scales) if a else None, stream_ptr()), "rownorm_fwd")
+                                     f, ptr(a.codes) if a else None, ptr(a.scales) if a else None, _lib.raw_stream(dev.index)), "rownorm_fwd")
     return y, mean, rstd, a
 
 
@@ -1631,7 +1644,7 @@ def rownorm_bwd(dy, saved, scale, mean, rstd, kind="layer", accum=None, want_par
     lda = 0
     if accum is not None:
         accum, _, _, lda = _rows_of(accum, "accum", dy)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+    dx = _like_rows(dy)
     dscale = torch.empty(C, dtype=F32, device=dev) if want_params else None
     doffset = torch.empty(C, dtype=F32, device=dev) if want_params else None
     if rows == 0:
@@ -1641,7 +1654,7 @@ def rownorm_bwd(dy, saved, scale, mean, rstd, kind="layer", accum=None, want_par
     nbytes = lib().dpig_rownorm_bwd_workspace_bytes(rows, C) if want_params else 0
     ws = _scratch(nbytes, dev)
     check(lib().dpig_rownorm_bwd(ptr(dy), int(dy.dtype == BF16), ld, xp, ldx, f, codes, scales, rows, C, k, ptr(scale), ptr(mean), ptr(rstd),
-                                 ptr(accum), lda, ptr(dx), C, ptr(dscale), ptr(doffset), ptr(ws), nbytes, stream_ptr()), "rownorm_bwd")
+                                 ptr(accum), lda, ptr(dx), C, ptr(dscale), ptr(doffset), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "rownorm_bwd")
     return dx, dscale, doffset
 
 
@@ -1673,7 +1686,7 @@ def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None,
     dev = x.device
     scale, offset, res_scale = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev), _chan(res_scale, C, "res_scale", dev)
     gate, groups = _gate_groups(gate, x, rows, C)
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    out = _like_rows(x)
     mean = torch.empty(rows, dtype=F32, device=dev) if k == 0 else None
     rstd = torch.empty(rows, dtype=F32, device=dev)
     a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
@@ -1684,7 +1697,7 @@ def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None,
         k2 = _kind(kind2)
         q2 = _fmt8(next_save8) if next_save8 is not None else 0
         scale2, offset2 = _chan(scale2, C, "the next norm's scale", dev), _chan(offset2, C, "the next norm's offset", dev)
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        h = _like_rows(x)
         mean2 = torch.empty(rows, dtype=F32, device=dev) if k2 == 0 else None
         rstd2 = torch.empty(rows, dtype=F32, device=dev)
         a2 = _new_act8(x.shape, rows, C, next_save8, dev) if next_save8 is not None else None
@@ -1695,7 +1708,7 @@ def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None,
             ptr(x), ldx, ptr(f), ldf, int(x.dtype == BF16), rows, C, k, ptr(scale), ptr(offset), eps, ptr(gate),
             int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(out), C, ptr(mean), ptr(rstd), q, ptr(a.codes) if a else None,
             ptr(a.scales) if a else None, k2, ptr(scale2), ptr(offset2), eps2, ptr(h), C, ptr(mean2), ptr(rstd2), q2,
-            ptr(a2.codes) if a2 else None, ptr(a2.scales) if a2 else None, stream_ptr()), "gated_residual_fwd")
+            ptr(a2.codes) if a2 else None, ptr(a2.scales) if a2 else None, _lib.raw_stream(dev.index)), "gated_residual_fwd")
     return out, mean, rstd, a, ((h, mean2, rstd2, a2) if next_norm is not None else None)
 
 
@@ -1711,7 +1724,7 @@ def gated_residual_bwd(dout, saved, scale, offset, gate, res_scale, mean, rstd, 
     mean, rstd = _row_stat(mean, rows, "mean", dev), _row_stat(rstd, rows, "rstd", dev)
     if rstd is None or (k == 0 and mean is None and fp is not None):
         raise RuntimeError("gated_residual_bwd: the statistics of the forward pass are needed")
-    df = torch.empty(dout.shape, dtype=dout.dtype, device=dev)
+    df = _like_rows(dout)
     dscale = doffset = dgate = dres = None
     if want_params:
         dscale = torch.empty(C, dtype=F32, device=dev)
@@ -1728,7 +1741,7 @@ def gated_residual_bwd(dout, saved, scale, offset, gate, res_scale, mean, rstd, 
     check(lib().dpig_gated_residual_bwd(
         ptr(dout), int(dout.dtype == BF16), ld, fp, ldf, q, codes, scales, rows, C, k, ptr(scale), ptr(offset), ptr(gate),
         int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(mean), ptr(rstd), ptr(df), C, ptr(dscale), ptr(doffset), ptr(dgate),
-        ptr(dres), ptr(ws), nbytes, stream_ptr()), "gated_residual_bwd")
+        ptr(dres), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "gated_residual_bwd")
     return df, dscale, doffset, dgate, dres
 
 

@@ -173,6 +173,34 @@ def test_linear_wgrad8_of_integers_is_exact(dev, rows, C, K, dtype):
     assert torch.equal(db.cpu().double(), dy.double().sum(0))
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C", [(128, 300), (131, 64), (640, 130)])
+def test_linear_wgrad8_reads_every_value_exactly(dev, rows, C, dtype, fmt):
+    """dy the identity: dw is the checkpoint's values transposed, whatever their sizes."""
+    H = _H()
+    g = torch.Generator().manual_seed(C)
+    x = torch.randn(rows, C, generator=g) * torch.exp(12 * torch.randn(rows, C, generator=g))
+    x[0, :8] = torch.tensor([3.4e38, -3.4e38, 1e-30, -1e-38, 1e-44, 0.0, 2.0 ** 127, -1.9 * 2.0 ** 126])
+    a = H.act8_store(x.to(dev), fmt)
+    dw, db = H.linear_wgrad8(a, torch.eye(rows, dtype=dtype, device=dev), want_bias=True)
+    assert torch.equal(dw.double().cpu(), R.checkpoint(x, fmt)[2].t().contiguous())
+    assert torch.equal(db.cpu(), torch.ones(rows))
+
+
+# the 256 x 128 and 256 x 256 tiles are taken from 2^32 and 2^35 products on (fp32 dy: a third of that)
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,C,K,dtype", [(33000, 250, 520, BF16), (133001, 500, 520, BF16), (133001, 512, 513, BF16), (40001, 200, 260, F32)])
+def test_linear_wgrad8_large_tiles_are_exact_on_integers(dev, rows, C, K, dtype, fmt):
+    H = _H()
+    g = torch.Generator(device=dev).manual_seed(rows)
+    q = torch.randint(-8, 9, (rows, C), generator=g, device=dev).float()        # (both formats hold these as they are)
+    dy = torch.randint(-3, 4, (rows, K), generator=g, device=dev)
+    dw, db = H.linear_wgrad8(H.act8_store(q, fmt), dy.to(dtype), want_bias=True)
+    want = q.double().t().contiguous() @ dy.double()
+    assert torch.equal(dw.double(), want) and torch.equal(db.double(), dy.double().sum(0))
+
+
 def test_linear_wgrad8_strides_and_not_finite_values(dev):
     H = _H()
     x, dy, _, _ = _operands(300, 70, 90, F32, "e4m3", 9)
