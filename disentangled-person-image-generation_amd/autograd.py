@@ -4,6 +4,7 @@ memory.  The gradient definitions are the ones TF autodiff derives for the refer
 (trainer.py:137-140).
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import hip_ops as H
 from ._lib import ACT_LRELU, ACT_NONE, ACT_RELU
@@ -319,6 +320,78 @@ def _sink_small(p, g):
     return None
 
 
+# ---- activations kept for the backward pass in 8 bits ---------------------------------------------------------------------------
+# With a format set, the conv / residual block / fully connected Functions keep hip_ops.Act8 checkpoints of their inputs and activation outputs
+# instead of the tensors: 33/32 bytes an element against 2 or 4 (a quarter of fp32's, half of bf16's where nobody else holds the tensor).
+# The backward pass reads them: activation masks and the filter gradients of 1x1 / fully connected layers directly, other filter gradients from
+# values decoded into a scratch tensor.  Forward results are unchanged; filter gradients see inputs rounded to 8 bits.
+SAVE8 = [None]
+
+
+def set_activation_checkpoint(fmt):
+    """'e4m3' | 'int8': subsequent forward passes keep their activations in 8 bits; None: as they are (the default)."""
+    if fmt is not None:
+        H._fmt8(fmt)
+    SAVE8[0] = fmt
+
+
+class _Kept8(object):
+    """A checkpoint with the type of the tensor it stands for."""
+    __slots__ = ("a", "dtype")
+
+    def __init__(self, t, fmt):
+        self.a, self.dtype = H.act8_store(t, fmt), t.dtype
+
+    @property
+    def shape(self):
+        return self.a.shape
+
+    def load(self):
+        return H.act8_load(self.a, self.dtype)
+
+    def act_bwd(self, dy, act, alpha=0.2):
+        dz = H.act8_act_bwd(dy, self.a, act, alpha)
+        if dz.dtype == self.dtype:
+            return dz
+        return H.to_bf16(dz) if self.dtype == H.BF16 else H.to_f32(dz)
+
+
+def _fmt_now(save8=None):
+    """The checkpoint format of a Function applied now: none where nothing will be differentiated."""
+    return (save8 if save8 is not None else SAVE8[0]) if torch.is_grad_enabled() else None
+
+
+def _worth8(t, fmt):
+    """Few channels stay as they are: a group of 32 pads them beyond what they save."""
+    return fmt is not None and t is not None and t.is_cuda and t.shape[-1] * t.element_size() * 3 >= 4 * (-(-t.shape[-1] // 32) * 33)
+
+
+def _keep(t, fmt):
+    """(tensor to save, checkpoint): one of the two is None."""
+    return (None, _Kept8(t, fmt)) if _worth8(t, fmt) else (t, None)
+
+
+def _sink_wgrad8(w, b, a, dz, want_w, want_b, scale=None, offset=None):
+    """Filter (+ bias) gradient of a product whose input is the checkpoint `a` (times scale plus offset), into the flat sinks where there are any."""
+    if not want_w:
+        return None, _sink(b, lambda o, beta: H.colsum(dz, out=o, beta=beta)) if want_b else None
+    wbuf = getattr(w, "_dpig_grad", None)
+    bbuf = getattr(b, "_dpig_grad", None) if want_b else None
+    wbeta = 1.0 if wbuf is not None and w._dpig_touched[0] else 0.0
+    bbeta = 1.0 if bbuf is not None and b._dpig_touched[0] else 0.0
+    r = H.linear_wgrad8(a, dz, scale, offset, out=wbuf, beta=wbeta, want_bias=want_b, db=bbuf, db_beta=bbeta)
+    dw, db = r if want_b else (r, None)
+    if wbuf is not None:
+        w._dpig_touched[0] = True
+        dw = None
+    elif dw is not None:
+        dw = dw.view(w.shape)
+    if bbuf is not None:
+        b._dpig_touched[0] = True
+        db = None
+    return dw, db
+
+
 # ---- second-level functions: the backward passes themselves, differentiable once more -------------
 # Used only when a backward pass runs with create_graph=True (the WGAN-GP penalty is a function of
 # dD/dx, trainer.py:222-236).  LeakyReLU/ReLU are piecewise linear, so nothing flows through the masks;
@@ -410,7 +483,7 @@ class _ConvFn(torch.autograd.Function):
     """y = act(conv_SAME(x, w) + b)   [optionally on a nearest-2x-upsampled x, 1x1 only]."""
 
     @staticmethod
-    def forward(ctx, x, w, b, stride, act, alpha, upsample2x, stats_box=None, out=None):
+    def forward(ctx, x, w, b, stride, act, alpha, upsample2x, stats_box=None, out=None, save8=None):
         if stats_box is not None and act == ACT_NONE and not upsample2x:
             # the caller's next op is a batch norm: let the conv epilogue leave the per-tile statistics (None when it cannot)
             y, st = H.conv2d_fwd_stats(x, w, b, stride=stride)
@@ -418,7 +491,10 @@ class _ConvFn(torch.autograd.Function):
         else:
             y = H.conv2d_fwd(x, w, b, stride=stride, act=act, alpha=alpha, upsample2x=upsample2x,
                              out=out.t if out is not None else None, emit32=True)      # (a conv's output mostly feeds a conv)
-        ctx.save_for_backward(x, w, y if act != ACT_NONE else None)
+        ctx.x_shape = tuple(x.shape)
+        x, ctx.x8 = _keep(x, save8)
+        y_kept, ctx.y8 = _keep(y, save8) if act != ACT_NONE else (None, None)
+        ctx.save_for_backward(x, w, y_kept)
         ctx.cfg = (stride, act, alpha, upsample2x, b is not None)
         ctx.b_ref = b
         return y
@@ -426,19 +502,32 @@ class _ConvFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         x, w, y = ctx.saved_tensors
+        x8, y8, x_shape = ctx.x8, ctx.y8, ctx.x_shape
         stride, act, alpha, up, has_b = ctx.cfg
         second = torch.is_grad_enabled()       # backward under create_graph=True
+        if y8 is not None and (second or up):
+            y, y8 = y8.load(), None
+
+        def filter_grads(dz, up):
+            want_w, want_b = ctx.needs_input_grad[1], has_b and ctx.needs_input_grad[2]
+            if x8 is None:
+                return _sink_wgrad_bias(w, ctx.b_ref, x, dz, stride, up, want_w, want_b)
+            if w.shape[0] == 1 and w.shape[1] == 1 and stride == 1 and not up:
+                return _sink_wgrad8(w, ctx.b_ref, x8.a, dz, want_w, want_b)
+            return _sink_wgrad_bias(w, ctx.b_ref, x8.load() if want_w else None, dz, stride, up, want_w, want_b)
         if up and not second and w.shape[0] == 1 and w.shape[1] == 1:
             # act(conv1x1(upsample2x(x))): nearest upsampling commutes with the 1x1 conv, so its gradient lives on x's grid:
             # one pass forms sum_{2x2} dy * act'(y) there, then plain 1x1 dgrad / wgrad (no 4-tap gathers of the 4x larger dy)
             dzp = H.act_bwd_pool2x(dy, y, act, alpha)
-            dx = H.conv2d_dgrad(dzp, w, tuple(x.shape), stride=1) if ctx.needs_input_grad[0] else None
+            dx = H.conv2d_dgrad(dzp, w, x_shape, stride=1) if ctx.needs_input_grad[0] else None
             if _PARAM_GRADS_OFF[0]:
-                return dx, None, None, None, None, None, None, None, None
-            dw, db = _sink_wgrad_bias(w, ctx.b_ref, x, dzp, 1, False, ctx.needs_input_grad[1], has_b and ctx.needs_input_grad[2])
-            return dx, dw, db, None, None, None, None, None, None
+                return dx, None, None, None, None, None, None, None, None, None
+            dw, db = filter_grads(dzp, False)
+            return dx, dw, db, None, None, None, None, None, None, None
         if second:
             dz = _ActBwdFn.apply(dy, y, act, alpha) if act != ACT_NONE else dy
+        elif y8 is not None:
+            dz = y8.act_bwd(dy, act, alpha)         # (a gradient that its consumer has masked already is masked again: the same)
         elif act == ACT_RELU and _premasked(dy, y):
             dz = dy                                 # the consuming residual block's dgrad already applied relu'(y)
         else:
@@ -446,15 +535,14 @@ class _ConvFn(torch.autograd.Function):
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             if second:
-                dx = _ConvDgradFn.apply(dz, w, tuple(x.shape), stride, up)
+                dx = _ConvDgradFn.apply(dz, w, x_shape, stride, up)
                 dz = dz.detach()
             else:
-                dx = H.conv2d_dgrad(dz, w, tuple(x.shape), stride=stride, upsample2x=up)
+                dx = H.conv2d_dgrad(dz, w, x_shape, stride=stride, upsample2x=up)
         if _PARAM_GRADS_OFF[0]:
-            return dx, None, None, None, None, None, None, None, None
-        dw, db = _sink_wgrad_bias(w, ctx.b_ref, x, dz, stride, up, ctx.needs_input_grad[1],
-                                  has_b and ctx.needs_input_grad[2])
-        return dx, dw, db, None, None, None, None, None, None
+            return dx, None, None, None, None, None, None, None, None, None
+        dw, db = filter_grads(dz, up)
+        return dx, dw, db, None, None, None, None, None, None, None
 
 
 def conv2d(x, w, b=None, stride=1, act=ACT_NONE, alpha=0.2, upsample2x=False, bn_stats=False, out=None):
@@ -463,10 +551,10 @@ def conv2d(x, w, b=None, stride=1, act=ACT_NONE, alpha=0.2, upsample2x=False, bn
     `out`: a channel slice of a wider NHWC buffer to write the result into (see `join_channels`)."""
     if not bn_stats:
         if out is not None:
-            return _ConvFn.apply(x, w, b, stride, act, alpha, upsample2x, None, _Out(out))
-        return _mark_relu_output(_ConvFn.apply(x, w, b, stride, act, alpha, upsample2x), act)
+            return _ConvFn.apply(x, w, b, stride, act, alpha, upsample2x, None, _Out(out), _fmt_now())
+        return _mark_relu_output(_ConvFn.apply(x, w, b, stride, act, alpha, upsample2x, None, None, _fmt_now()), act)
     box = []
-    y = _ConvFn.apply(x, w, b, stride, act, alpha, upsample2x, box)
+    y = _ConvFn.apply(x, w, b, stride, act, alpha, upsample2x, box, None, _fmt_now())
     if box and box[0] is not None:
         y._dpig_bnstats = box[0]
     return y
@@ -479,13 +567,18 @@ class _ResBlockFn(torch.autograd.Function):
     dgrad(conv2) applies c1's ReLU mask and dgrad(conv1) adds the skip gradient in its epilogue."""
 
     @staticmethod
-    def forward(ctx, x0, w1, b1, w2, b2, out=None):
+    def forward(ctx, x0, w1, b1, w2, b2, out=None, save8=None):
         ctx.x0_relu = bool(getattr(x0, "_dpig_relu_out", False))
         c1 = H.conv2d_fwd(x0, w1, b1, act=ACT_RELU, emit32=True)
         c2 = torch.empty_like(c1)
         out = torch.empty_like(c1) if out is None else out.t
         H.conv2d_fwd(c1, w2, b2, act=ACT_RELU, residual=x0, res_after_act=True, out=out, out_act=c2, emit32=True)
-        ctx.save_for_backward(x0, w1, w2, c1, c2)
+        ctx.k8 = None
+        if _worth8(x0, save8):
+            ctx.k8 = tuple(_Kept8(t, save8) for t in (x0, c1, c2))
+            ctx.save_for_backward(None, w1, w2, None, None)
+        else:
+            ctx.save_for_backward(x0, w1, w2, c1, c2)
         ctx.b_refs = (b1, b2)
         return out
 
@@ -493,26 +586,34 @@ class _ResBlockFn(torch.autograd.Function):
     def backward(ctx, dout):
         x0, w1, w2, c1, c2 = ctx.saved_tensors
         b1, b2 = ctx.b_refs
-        dz2 = H.act_bwd(dout, c2, ACT_RELU, emit32=True)
+        if ctx.k8 is not None:
+            x8, c18, c28 = ctx.k8
+            dz2 = c28.act_bwd(dout, ACT_RELU)
+            c1 = c18.load()                         # (values for the filter gradient, signs for the mask)
+        else:
+            dz2 = H.act_bwd(dout, c2, ACT_RELU, emit32=True)
         dw2, db2 = _sink_wgrad_bias(w2, b2, c1, dz2, want_w=ctx.needs_input_grad[3], want_b=ctx.needs_input_grad[4])
         dz1 = H.conv2d_dgrad(dz2, w2, tuple(c1.shape), mask=c1, act=ACT_RELU, emit32=True)    # feeds dgrad(conv1)
+        if ctx.k8 is not None:
+            del c1
+            x0 = x8.load()
         dw1, db1 = _sink_wgrad_bias(w1, b1, x0, dz1, want_w=ctx.needs_input_grad[1], want_b=ctx.needs_input_grad[2])
         dx0 = None
         if ctx.needs_input_grad[0]:
-            if ctx.x0_relu and FUSE_INPUT_MASK[0] and not torch.is_grad_enabled():
+            if ctx.x0_relu and FUSE_INPUT_MASK[0] and not torch.is_grad_enabled() and ctx.k8 is None:
                 # x0 is a ReLU conv's output: hand its producer the gradient w.r.t. the PRE-activation (mask in this epilogue)
                 dx0 = H.conv2d_dgrad(dz1, w1, tuple(x0.shape), accum=dout, mask=x0, act=ACT_RELU)
                 dx0._dpig_masked_for = (x0.data_ptr(), dx0._version)
             else:
                 dx0 = H.conv2d_dgrad(dz1, w1, tuple(x0.shape), accum=dout)
-        return dx0, dw1, db1, dw2, db2, None
+        return dx0, dw1, db1, dw2, db2, None, None
 
 
 def resblock(x0, w1, b1, w2, b2, out=None):
     """`out`: a channel slice of a wider NHWC buffer to write the block's output into (see `join_channels`)."""
     if out is not None:
-        return _ResBlockFn.apply(x0, w1, b1, w2, b2, _Out(out))
-    return _ResBlockFn.apply(x0, w1, b1, w2, b2)
+        return _ResBlockFn.apply(x0, w1, b1, w2, b2, _Out(out), _fmt_now())
+    return _ResBlockFn.apply(x0, w1, b1, w2, b2, None, _fmt_now())
 
 
 class _Out(object):
@@ -784,9 +885,12 @@ def conv2d_transpose(x, w, b=None):
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, b, act, alpha):
+    def forward(ctx, x, w, b, act, alpha, save8=None):
         y = H.linear_fwd(x, w, b, act=act, alpha=alpha)
-        ctx.save_for_backward(x, w, y if act != ACT_NONE else None)
+        ctx.x_dtype = x.dtype
+        x, ctx.x8 = _keep(x, save8)
+        y_kept, ctx.y8 = _keep(y, save8) if act != ACT_NONE else (None, None)
+        ctx.save_for_backward(x, w, y_kept)
         ctx.cfg = (act, alpha, b is not None)
         ctx.b_ref = b
         return y
@@ -796,27 +900,157 @@ class _LinearFn(torch.autograd.Function):
         x, w, y = ctx.saved_tensors
         act, alpha, has_b = ctx.cfg
         if torch.is_grad_enabled():            # backward under create_graph=True
+            if ctx.y8 is not None:
+                y = ctx.y8.load()
             dz = _ActBwdFn.apply(dy, y, act, alpha) if act != ACT_NONE else dy.contiguous()
             dx = _LinearDgradFn.apply(dz, w) if ctx.needs_input_grad[0] else None
             dz = dz.detach()
         else:
-            dz = H.act_bwd(dy, y, act, alpha) if act != ACT_NONE else dy.contiguous()
+            if ctx.y8 is not None:
+                dz = ctx.y8.act_bwd(dy, act, alpha)
+            else:
+                dz = H.act_bwd(dy, y, act, alpha) if act != ACT_NONE else dy.contiguous()
             dx = H.linear_dgrad(dz, w) if ctx.needs_input_grad[0] else None
         dw = db = None
-        if ctx.needs_input_grad[1] and not _PARAM_GRADS_OFF[0]:
-            dw = _sink(w, lambda o, beta: H.linear_wgrad(x, dz, out=o, beta=beta))
-        if has_b and ctx.needs_input_grad[2] and not _PARAM_GRADS_OFF[0]:
-            db = _sink(ctx.b_ref, lambda o, beta: H.colsum(dz, out=o, beta=beta))
-        if dx is not None and dx.dtype != x.dtype:
+        want_w = ctx.needs_input_grad[1] and not _PARAM_GRADS_OFF[0]
+        want_b = has_b and ctx.needs_input_grad[2] and not _PARAM_GRADS_OFF[0]
+        if ctx.x8 is not None:
+            dw, db = _sink_wgrad8(w, ctx.b_ref, ctx.x8.a, dz, want_w, want_b)
+        else:
+            if want_w:
+                dw = _sink(w, lambda o, beta: H.linear_wgrad(x, dz, out=o, beta=beta))
+            if want_b:
+                db = _sink(ctx.b_ref, lambda o, beta: H.colsum(dz, out=o, beta=beta))
+        if dx is not None and dx.dtype != ctx.x_dtype:
             if torch.is_grad_enabled():        # (on the tape: the penalty's gradient w.r.t. `w` flows back through this conversion)
-                dx = _CastFn.apply(dx, x.dtype == H.BF16)
+                dx = _CastFn.apply(dx, ctx.x_dtype == H.BF16)
             else:
-                dx = H.to_bf16(dx) if x.dtype == H.BF16 else H.to_f32(dx)
-        return dx, dw, db, None, None
+                dx = H.to_bf16(dx) if ctx.x_dtype == H.BF16 else H.to_f32(dx)
+        return dx, dw, db, None, None, None
 
 
-def linear(x, w, b=None, act=ACT_NONE, alpha=0.2):
-    return _LinearFn.apply(x, w, b, act, alpha)
+def linear(x, w, b=None, act=ACT_NONE, alpha=0.2, save8=None):
+    """`save8` ('e4m3' | 'int8'): keep x (and y, for the activation's mask) in 8 bits for the backward pass; default `set_activation_checkpoint`."""
+    return _LinearFn.apply(x, w, b, act, alpha, _fmt_now(save8))
+
+
+# ---- residual blocks on rows of channels (hip_ops.rownorm_* / gated_residual_* / Act8) --------------------------------------------------
+class _RowNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, scale, offset, eps, kind, save8):
+        y, mean, rstd, a = H.rownorm_fwd(x, scale, offset, eps, kind, save8=save8)
+        ctx.a, ctx.kind, ctx.offset_ref = a, kind, offset
+        ctx.save_for_backward(None if a is not None else x, scale, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, scale, mean, rstd = ctx.saved_tensors
+        off = _PARAM_GRADS_OFF[0]
+        want_s, want_o = ctx.needs_input_grad[1] and not off, ctx.needs_input_grad[2] and not off
+        dx, ds, do = H.rownorm_bwd(dy, ctx.a if x is None else x, scale, mean, rstd, ctx.kind, want_params=want_s or want_o)
+        return (dx, _sink_small(scale, ds) if want_s else None, _sink_small(ctx.offset_ref, do) if want_o else None, None, None, None)
+
+
+def rownorm(x, scale=None, offset=None, eps=1e-5, kind="layer", save8=None):
+    """Layer / RMS norm over the last axis.  First-order gradients.  `save8`: keep the normed values in 8 bits instead of x (default
+    `set_activation_checkpoint`)."""
+    return _RowNormFn.apply(x, scale, offset, eps, kind, _fmt_now(save8))
+
+
+class _GatedResidualFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, f, scale, offset, gate, res_scale, eps, kind, save8):
+        out, mean, rstd, a, _ = H.gated_residual_fwd(x, f, scale, offset, gate, res_scale, eps, kind, save8=save8)
+        ctx.a, ctx.kind = a, kind
+        ctx.refs = (scale, offset, res_scale)
+        ctx.save_for_backward(None if a is not None else f, scale, offset, gate, res_scale, mean, rstd)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        f, scale, offset, gate, res_scale, mean, rstd = ctx.saved_tensors
+        need, off = ctx.needs_input_grad, _PARAM_GRADS_OFF[0]
+        want = need[4] or (not off and (need[2] or need[3] or need[5]))
+        df, ds, do, dg, dr = H.gated_residual_bwd(dout, ctx.a if f is None else f, scale, offset, gate, res_scale, mean, rstd, ctx.kind, want_params=want)
+        sink = [_sink_small(p, g) if n and not off else None for p, g, n in zip(ctx.refs, (ds, do, dr), (need[2], need[3], need[5]))]
+        return (dout if need[0] else None, df if need[1] else None, sink[0], sink[1], dg.view(gate.shape) if need[4] else None, sink[2],
+                None, None, None)
+
+
+def gated_residual(x, f, scale=None, offset=None, gate=None, res_scale=None, eps=1e-5, kind="layer", save8=None):
+    """x + res_scale * gate * (scale * norm(f) + offset) over the last axis (hip_ops.gated_residual_fwd).  First-order gradients."""
+    return _GatedResidualFn.apply(x, f, scale, offset, gate, res_scale, eps, kind, _fmt_now(save8))
+
+
+class _GatedBlockFn(torch.autograd.Function):
+    """One residual block of fully connected layers on rows of channels:
+         h = norm(x) s1 + o1;  u = act(h w1 + b1);  f = u w2 + b2;  out = x + res_scale * gate * (norm(f) s2 + o2)
+    Without `save8` x, h, u and f are kept for the backward pass; with it their 8-bit checkpoints: one of the normed x, which serves the norm's
+    gradient and, through scale and offset, w1's; one of u, for w2's and for the activation's mask; one of the normed f."""
+
+    @staticmethod
+    def forward(ctx, x, s1, o1, w1, b1, w2, b2, s2, o2, gate, res_scale, act, alpha, eps, kind, save8):
+        h, m1, r1, x8 = H.rownorm_fwd(x, s1, o1, eps, kind, save8=save8)
+        C = x.shape[-1]
+        u = H.linear_fwd(h.reshape(-1, C), w1, b1, act=act, alpha=alpha)
+        u8 = H.act8_store(u, save8) if save8 is not None else None
+        f = H.linear_fwd(u, w2, b2)
+        f = (H.to_bf16(f) if x.dtype == H.BF16 else f).view(x.shape)
+        out, m2, r2, f8, _ = H.gated_residual_fwd(x, f, s2, o2, gate, res_scale, eps, kind, save8=save8)
+        ctx.kept8 = (x8, u8, f8)
+        keep = (None, None, None, None) if save8 is not None else (x, h, u, f)
+        ctx.save_for_backward(*keep, s1, o1, w1, w2, s2, o2, gate, res_scale, m1, r1, m2, r2)
+        ctx.refs = (s1, o1, b1, b2, s2, o2, res_scale)
+        ctx.cfg = (act, alpha, kind)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, h, u, f, s1, o1, w1, w2, s2, o2, gate, res_scale, m1, r1, m2, r2 = ctx.saved_tensors
+        x8, u8, f8 = ctx.kept8
+        rs1, ro1, b1, b2, rs2, ro2, rres = ctx.refs
+        act, alpha, kind = ctx.cfg
+        off = _PARAM_GRADS_OFF[0]
+        need = [n and (k in (0, 9) or not off) for k, n in enumerate(ctx.needs_input_grad)]
+        C = dout.shape[-1]
+        df, ds2, do2, dg, dr = H.gated_residual_bwd(dout, f8 if f is None else f, s2, o2, gate, res_scale, m2, r2, kind,
+                                                    want_params=any(need[k] for k in (7, 8, 9, 10)))
+        df = df.reshape(-1, C)
+        if u8 is not None:
+            dw2, db2 = _sink_wgrad8(w2, b2, u8, df, need[5], b2 is not None and need[6])
+        else:
+            dw2 = _sink(w2, lambda o, beta: H.linear_wgrad(u, df, out=o, beta=beta)) if need[5] else None
+            db2 = _sink(b2, lambda o, beta: H.colsum(df, out=o, beta=beta)) if b2 is not None and need[6] else None
+        du = H.linear_dgrad(H.to_f32(df), w2)
+        if act == ACT_NONE:
+            dz = du
+        else:
+            dz = H.act8_act_bwd(du, u8, act, alpha) if u8 is not None else H.act_bwd(du, u, act, alpha)
+        if x8 is not None:
+            dw1, db1 = _sink_wgrad8(w1, b1, x8, dz, need[3], b1 is not None and need[4], s1, o1)
+        else:
+            dw1 = _sink(w1, lambda o, beta: H.linear_wgrad(h.reshape(-1, C), dz, out=o, beta=beta)) if need[3] else None
+            db1 = _sink(b1, lambda o, beta: H.colsum(dz, out=o, beta=beta)) if b1 is not None and need[4] else None
+        dx = ds1 = do1 = None
+        if need[0] or need[1] or need[2]:
+            dh = H.linear_dgrad(dz, w1)
+            dh = (H.to_bf16(dh) if dout.dtype == H.BF16 else dh).view(dout.shape)
+            dx, ds1, do1 = H.rownorm_bwd(dh, x8 if x is None else x, s1, m1, r1, kind, accum=dout, want_params=need[1] or need[2])
+
+        def sink(p, g, k):
+            return _sink_small(p, g) if need[k] and g is not None else None
+        return (dx if need[0] else None, sink(rs1, ds1, 1), sink(ro1, do1, 2), dw1, db1, dw2, db2, sink(rs2, ds2, 7), sink(ro2, do2, 8),
+                dg.view(gate.shape) if need[9] else None, sink(rres, dr, 10), None, None, None, None, None)
+
+
+def gated_resblock(x, s1, o1, w1, b1, w2, b2, s2, o2, gate=None, res_scale=None, act=ACT_RELU, alpha=0.2, eps=1e-5, kind="layer", save8=None):
+    """`_GatedBlockFn`.  x [..., C] fp32 or bf16, w1 [C, F], w2 [F, C], fp32 parameters; gate as hip_ops.gated_residual_fwd.  First-order gradients.
+    `save8`: default `set_activation_checkpoint`."""
+    return _GatedBlockFn.apply(x, s1, o1, w1, b1, w2, b2, s2, o2, gate, res_scale, act, alpha, eps, kind, _fmt_now(save8))
 
 
 class _BatchNormFn(torch.autograd.Function):

@@ -120,6 +120,14 @@ __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) { a[j][e] *= t[e]; b[j][e] *= t[e]; m[j][e] = 1.f; }
     }
+    float sc2[NEXT ? NV : 1][8], of2[NEXT ? NV : 1][8];
+    if (NEXT) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            ldp(p.scale2, 8 * (lane + LPR * j), p.C, 1.f, sc2[j]);
+            ldp(p.offset2, 8 * (lane + LPR * j), p.C, 0.f, of2[j]);
+        }
+    }
     long g = EACH || p.gate == nullptr ? 0 : r / p.per, until = p.gate == nullptr ? p.nrows : (g + 1) * p.per;     // r's group, and its end
     if (!EACH && p.gate != nullptr && r < r1) {
 #pragma unroll
@@ -172,13 +180,9 @@ __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
             if (p.save2.codes != nullptr) save8<LPR, NV>(p.save2, r, lane, v);
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int c = 8 * (lane + LPR * j);
-                float sc[8], of[8];
-                ldp(p.scale2, c, p.C, 1.f, sc);
-                ldp(p.offset2, c, p.C, 0.f, of);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], sc[e], of[e]);
-                st8<RAG>(static_cast<T*>(p.h) + r * p.ldh + c, v[j], n[j]);
+                for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], sc2[j][e], of2[j][e]);
+                st8<RAG>(static_cast<T*>(p.h) + r * p.ldh + 8 * (lane + LPR * j), v[j], n[j]);
             }
         }
     }

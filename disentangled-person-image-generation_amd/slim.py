@@ -143,8 +143,35 @@ def res_block(inputs, channel_num, kernel_size=3, activation_fn=relu, data_forma
     return x + inputs
 
 
-def fully_connected(inputs, num_outputs, activation_fn=relu, scope=None):
-    """slim.fully_connected(x, n, activation_fn=...) (models.py:431,464,545,554; FC nets 474-515)."""
+def gated_res_block(inputs, num_hidden=None, gate=None, activation_fn=relu, kind="layer", eps=1e-5, save8=None, scope=None):
+    """The fully connected residual block of models.py:474-515 (x + fc(fc(x))) with a norm over the channels before and after, a gate and a learned
+    residual scale (beyond the reference):
+        x + res_scale * gate * (norm(fc(act(fc(norm(x) * s1 + o1)))) * s2 + o2)
+    inputs [..., C] (rows of channels), `num_hidden` the inner width (default C), gate [C], [G, C] or as inputs (None: 1), e.g. a fully_connected
+    of a conditioning vector.  Variables `<scope>/GatedResidual[_k]/{entry_scale, entry_offset, exit_scale, exit_offset, res_scale}` and two
+    `fully_connected[_k]/{weights, biases}`; res_scale starts at 0.1.  `save8` ('e4m3' | 'int8'): activations kept in 8 bits for the
+    backward pass."""
+    act, foreign = _act_code(activation_fn)
+    if foreign is not None:
+        raise Exception("gated_res_block takes relu, leaky_relu or no activation")
+    C = inputs.shape[-1]
+    F = C if num_hidden is None else num_hidden
+    name = scope if scope is not None else _unique("GatedResidual")
+    n1, n2 = _unique("fully_connected"), _unique("fully_connected")
+
+    def var(leaf, value):
+        return lib.param(name + "/" + leaf, np.full(C, value, dtype="float32"))
+    s1, o1 = var("entry_scale", 1.0), var("entry_offset", 0.0)
+    w1 = lib.param(n1 + "/weights", None if n1 + "/weights" in lib._params else _xavier_uniform((C, F), C, F))
+    b1 = lib.param(n1 + "/biases", np.zeros(F, dtype="float32"))
+    w2 = lib.param(n2 + "/weights", None if n2 + "/weights" in lib._params else _xavier_uniform((F, C), F, C))
+    b2 = lib.param(n2 + "/biases", np.zeros(C, dtype="float32"))
+    s2, o2, res = var("exit_scale", 1.0), var("exit_offset", 0.0), var("res_scale", 0.1)
+    return A.gated_resblock(inputs, s1, o1, w1, b1, w2, b2, s2, o2, gate, res, act, 0.2, eps, kind, save8)
+
+
+def fully_connected(inputs, num_outputs, activation_fn=relu, scope=None, save8=None):
+    """slim.fully_connected(x, n, activation_fn=...) (models.py:431,464,545,554; FC nets 474-515).  `save8` (extension): see autograd.linear."""
     name = scope if scope is not None else _unique("fully_connected")
     cin = inputs.shape[-1]
     wname = name + "/weights"
@@ -152,6 +179,6 @@ def fully_connected(inputs, num_outputs, activation_fn=relu, scope=None):
     w = lib.param(wname, w_init)
     b = lib.param(name + "/biases", np.zeros(num_outputs, dtype="float32"))
     act, foreign = _act_code(activation_fn)
-    y = A.linear(inputs.reshape(-1, cin), w, b, act)
+    y = A.linear(inputs.reshape(-1, cin), w, b, act, save8=save8)
     y = y.reshape(tuple(inputs.shape[:-1]) + (num_outputs,))
     return foreign(y) if foreign is not None else y

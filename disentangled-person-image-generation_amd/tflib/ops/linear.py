@@ -27,10 +27,11 @@ def unset_weights_stdev():
 
 
 def Linear(name, input_dim, output_dim, inputs, biases=True, initialization=None, weightnorm=None, gain=1.,
-           fused_act=None, alpha=0.2):
+           fused_act=None, alpha=0.2, save8=None):
     """initialization: None (Glorot), 'lecun', 'glorot', 'he', 'glorot_he', 'orthogonal' or ('uniform', range).
     `fused_act` in {None,'relu','lrelu'} (extension) folds the caller's next activation into the GEMM epilogue.
-    Inputs of any rank: the last axis is the feature axis."""
+    Inputs of any rank: the last axis is the feature axis.  `save8` ('e4m3' | 'int8', extension): inputs kept in 8 bits for the
+    backward pass."""
     fresh = None
     if name + '.W' not in lib._params:
         fresh = _init.linear_weight_values(_SW, initialization, input_dim, output_dim, gain)
@@ -39,5 +40,6 @@ def Linear(name, input_dim, output_dim, inputs, biases=True, initialization=None
         W = _init.weight_normalised(name, W, fresh, reduce_axes=0)
     b = _init.zero_bias(name + '.b', (output_dim,)) if biases else None
     lead = tuple(inputs.shape[:-1])
-    y = A.linear(inputs.reshape(-1, input_dim) if inputs.dim() != 2 else inputs, W, b, _ACT[fused_act], alpha)
+    y = A.linear(inputs.reshape(-1, input_dim) if inputs.dim() != 2 else inputs, W, b, _ACT[fused_act], alpha,
+                 save8=save8)
     return y if inputs.dim() == 2 else y.reshape(lead + (output_dim,))

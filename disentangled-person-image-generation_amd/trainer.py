@@ -388,6 +388,7 @@ class Config(object):
                                          # activations / their gradients / filter shadows stored as bf16, bf16 matrix
                                          # pipe, fp32 accumulation, master weights, gradients and optimizer.  'bf16c':
                                          # fp32 tensors, conv operands rounded to bf16 (hip_ops module docstring)
+        self.act_checkpoint = None       # 'e4m3' | 'int8': activations kept for the backward pass in 8 bits (autograd.set_activation_checkpoint)
         self.pretrained_path = None      # V2 checkpoint prefixes (trainer.py:180-212): 'Encoder' + 'ID_AE' variables,
         self.pretrained_poseAE_path = None   # the 'PoseAE' variables,
         self.ckpt_path = None            # every variable of the model
@@ -472,6 +473,7 @@ class DPIG_Encoder_GAN_BodyROI_FgBg(object):
     def init_net(self, batch):
         """Create every variable (one forward, like TF graph construction) and set up optimizers."""
         H.set_compute(getattr(self.config, "compute_dtype", "f32"))
+        A.set_activation_checkpoint(getattr(self.config, "act_checkpoint", None))
         with torch.no_grad():
             embs, enc_var = self.encode(batch)
             G, g_var = self.generate(embs, pose_input(batch, self.img_H, self.img_W))
@@ -708,6 +710,7 @@ class DPIG_Encoder_GAN_BodyROI_FgBg(object):
 
     def _g_forward(self, batch):
         H.set_compute(getattr(self.config, "compute_dtype", "f32"))
+        A.set_activation_checkpoint(getattr(self.config, "act_checkpoint", None))
         self.G_flat.zero_grad()
         self.D_flat.set_requires_grad(False)
         embs, _ = self.encode(batch)
@@ -833,6 +836,7 @@ class DPIG_Encoder_GAN_BodyROI_FgBg(object):
     def _d_optim_eager(self, batch, update=True):
         """sess.run(d_optim): fwd E,G (no grad), D(x), D(G); d_loss; bwd D; Adam(D)."""
         H.set_compute(getattr(self.config, "compute_dtype", "f32"))
+        A.set_activation_checkpoint(getattr(self.config, "act_checkpoint", None))
         self.D_flat.zero_grad()
         if (A.D_OVERLAP[0] and self.wgan_gp.MODE == 'dcgan' and batch["x"].is_cuda and not self._sync_bn_active()
                 and type(self).disc_pair is DPIG_Encoder_GAN_BodyROI_FgBg.disc_pair):        # (SyncBN's collectives cannot sit inside a forked stream of a capture)

@@ -72,6 +72,7 @@ class DPIG_Encoder_subSampleAppNet_GAN_BodyROI_256(object):
 
     def encode(self, batch):
         H.set_compute(getattr(self.config, "compute_dtype", "f32"))
+        A.set_activation_checkpoint(getattr(self.config, "act_checkpoint", None))
         with torch.no_grad(), slim.variable_scope("Encoder"):
             embs, _, enc_var = models.GeneratorCNN_ID_Encoder_BodyROI(
                 batch["x"], batch["part_bbox"], self.part_num, 32, self.repeat_num + 1, self.conv_hidden_num,

@@ -50,6 +50,7 @@ class DPIG_Encoder_subSampleAppNetFgBg_GAN_BodyROI(object):
     def encode(self, batch):
         """Frozen stage-I encoder (restored from --pretrained_path in the reference, trainer.py:180-183)."""
         H.set_compute(getattr(self.config, "compute_dtype", "f32"))
+        A.set_activation_checkpoint(getattr(self.config, "act_checkpoint", None))
         with torch.no_grad(), slim.variable_scope("Encoder"):
             embs, _, _, enc_var = models.GeneratorCNN_ID_Encoder_BodyROIVis_FgBgFeaTwoBranch(
                 batch["x"], batch["mask_r6"], batch["part_bbox"], batch["part_vis"], self.part_num, 32,

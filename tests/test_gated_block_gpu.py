@@ -1,0 +1,266 @@
+"""The residual-block operators as a user has them: the gated block, 8-bit checkpoints in the framework's own conv / residual / fully connected layers,
+and a training step with them."""
+import numpy as np
+import pytest
+import torch
+
+import rows_reference as R
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _mods():
+    import dpig_amd.autograd as A
+    import dpig_amd.hip_ops as H
+    return A, H
+
+
+@pytest.fixture(autouse=True)
+def _no_checkpoints_left_on():
+    yield
+    _mods()[0].set_activation_checkpoint(None)
+
+
+def _params(C, F, seed):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)     # noqa: E731
+    return dict(s1=1 + 0.1 * n(C), o1=0.1 * n(C), w1=n(C, F) / C ** 0.5, b1=0.1 * n(F), w2=n(F, C) / F ** 0.5, b2=0.1 * n(C), s2=1 + 0.1 * n(C),
+                o2=0.1 * n(C), res=0.5 + 0.1 * n(C))
+
+
+def _block64(x, p, gate, kind, act):
+    def norm(t):
+        m = t.mean(-1, keepdim=True) if kind == "layer" else 0.0
+        return (t - m) / torch.sqrt(((t - m) ** 2).mean(-1, keepdim=True) + 1e-5)
+    u = (norm(x) * p["s1"] + p["o1"]) @ p["w1"] + p["b1"]
+    u = torch.relu(u) if act == 1 else torch.where(u > 0, u, 0.2 * u)
+    f = u @ p["w2"] + p["b2"]
+    return x + p["res"] * gate * (norm(f) * p["s2"] + p["o2"])
+
+
+ORDER = ("s1", "o1", "w1", "b1", "w2", "b2", "s2", "o2")
+
+
+@pytest.mark.parametrize("kind,act", [("layer", 1), ("rms", 2)])
+@pytest.mark.parametrize("shape,F", [((64, 128), 128), ((2, 3, 5, 40), 96), ((1, 33), 17)])
+def test_block_and_its_gradients(dev, shape, F, kind, act):
+    """Against float64 autograd.  The products run over at most 128 terms and the norms' statistics over as many: 2e-5 of each tensor's largest value
+    is 300 fp32 half-steps, where a product's worst case is about 130 and the chain has six of them that mostly do not meet in one element."""
+    A, H = _mods()
+    C = shape[-1]
+    p = _params(C, F, 1)
+    g = torch.Generator().manual_seed(2)
+    x, gate, dy = torch.randn(shape, generator=g), 1 + 0.3 * torch.randn(shape, generator=g), torch.randn(shape, generator=g)
+    leaves = {k: v.clone().to(dev).requires_grad_(True) for k, v in list(p.items()) + [("x", x), ("gate", gate)]}
+    out = A.gated_resblock(leaves["x"], *[leaves[k] for k in ORDER], leaves["gate"], leaves["res"], act, 0.2, 1e-5, kind)
+    out.backward(dy.to(dev))
+    ref = {k: v.detach().double().cpu().requires_grad_(True) for k, v in leaves.items()}
+    r = _block64(ref["x"], ref, ref["gate"], kind, act)
+    r.backward(dy.double())
+    assert float((out.double().cpu() - r).abs().max()) <= 2e-5 * float(r.detach().abs().max())
+    for k, v in leaves.items():
+        want = ref[k].grad
+        assert v.grad.shape == want.shape
+        assert float((v.grad.double().cpu() - want).abs().max()) <= 2e-5 * max(float(want.abs().max()), 1e-2), k
+    with pytest.raises(RuntimeError):                     # (second-order gradients are refused, not wrong)
+        y = A.gated_resblock(leaves["x"], *[leaves[k] for k in ORDER], leaves["gate"], leaves["res"], act, 0.2, 1e-5, kind)
+        d, = torch.autograd.grad(y.sum(), leaves["x"], create_graph=True)
+        d.sum().backward()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_block_with_checkpoints_is_the_run_of_its_operators(dev, dtype, fmt, kind):
+    """save8 changes no forward bit, and the gradients are those of the operators called one after the other on the checkpoints."""
+    A, H = _mods()
+    N, C, F = 96, 72, 160
+    p = {k: v.to(dev) for k, v in _params(C, F, 3).items()}
+    g = torch.Generator().manual_seed(4)
+    x, dy = torch.randn(N, C, generator=g).to(dtype).to(dev), torch.randn(N, C, generator=g).to(dtype).to(dev)
+    gate = (1 + 0.3 * torch.randn(8, C, generator=g)).to(dev)
+    plain = A.gated_resblock(x, *[p[k] for k in ORDER], gate, p["res"], 1, 0.2, 1e-5, kind)
+    leaves = {k: v.clone().requires_grad_(True) for k, v in list(p.items()) + [("x", x), ("gate", gate)]}
+    out = A.gated_resblock(leaves["x"], *[leaves[k] for k in ORDER], leaves["gate"], leaves["res"], 1, 0.2, 1e-5, kind, save8=fmt)
+    assert torch.equal(out, plain)
+    out.backward(dy)
+    h, m1, r1, x8 = H.rownorm_fwd(x, p["s1"], p["o1"], 1e-5, kind, save8=fmt)
+    u = H.linear_fwd(h, p["w1"], p["b1"], act=1)
+    u8 = H.act8_store(u, fmt)
+    f = H.linear_fwd(u, p["w2"], p["b2"])
+    f = H.to_bf16(f) if dtype == BF16 else f
+    _, m2, r2, f8, _ = H.gated_residual_fwd(x, f, p["s2"], p["o2"], gate, p["res"], 1e-5, kind, save8=fmt)
+    df, ds2, do2, dg, dr = H.gated_residual_bwd(dy, f8, p["s2"], p["o2"], gate, p["res"], m2, r2, kind)
+    dw2, db2 = H.linear_wgrad8(u8, df, want_bias=True)
+    dz = H.act8_act_bwd(H.linear_dgrad(H.to_f32(df), p["w2"]), u8, 1)
+    assert torch.equal(dz == 0, (u == 0) | (dz == 0))      # the mask is u's own
+    dw1, db1 = H.linear_wgrad8(x8, dz, p["s1"], p["o1"], want_bias=True)
+    dh = H.linear_dgrad(dz, p["w1"])
+    dx, ds1, do1 = H.rownorm_bwd(H.to_bf16(dh) if dtype == BF16 else dh, x8, p["s1"], m1, r1, kind, accum=dy)
+    want = dict(x=dx, s1=ds1, o1=do1, w1=dw1, b1=db1, w2=dw2, b2=db2, s2=ds2, o2=do2, gate=dg, res=dr)
+    for k, v in want.items():
+        assert torch.equal(leaves[k].grad, v), k
+
+
+def test_single_functions_and_the_registry_layers(dev):
+    """rownorm / gated_residual under autograd, tflib's Rownorm, slim.gated_res_block (variables, scopes, leading axes) and Linear(save8=...)."""
+    A, H = _mods()
+    import dpig_amd.tflib as lib
+    import dpig_amd.tflib.ops  # noqa: F401
+    from dpig_amd import slim
+    lib.delete_all_params(); slim.reset_scopes(); lib.set_device(dev)
+    np.random.seed(0)
+    x = torch.randn(4, 6, 48, device=dev, requires_grad=True)
+    for save8 in (None, "int8"):
+        y = lib.ops.rownorm.Rownorm("N.%s" % save8, x, kind="layer", save8=save8)
+        gx, = torch.autograd.grad(y.square().sum(), x)
+        x64 = x.detach().double().cpu().requires_grad_(True)
+        m = x64.mean(-1, keepdim=True)
+        y64 = (x64 - m) / torch.sqrt(((x64 - m) ** 2).mean(-1, keepdim=True) + 1e-5)
+        g64, = torch.autograd.grad(y64.square().sum(), x64)
+        # (this loss is nearly flat: xh^2 sums to C whatever x is; what is left has the size of rounding times 2 xh rstd)
+        assert float((y.double().cpu() - y64).abs().max()) < 1e-5
+        assert float((gx.double().cpu() - g64).abs().max()) < (1e-4 if save8 is None else 0.2)
+    assert len(lib.params_with_name("N.int8")) == 2
+    with slim.variable_scope("Emb"):
+        gate = slim.fully_connected(torch.randn(4, 10, device=dev), 48, activation_fn=None)
+        a = slim.gated_res_block(x, 64, gate=gate.reshape(4, 1, 48), save8="e4m3")
+        b = slim.gated_res_block(a, gate=gate.reshape(4, 1, 48), kind="rms", activation_fn=slim.leaky_relu)
+    b.square().mean().backward()
+    names = sorted(n for n in lib._params if n.startswith("Emb/"))
+    assert [n for n in names if "Gated" in n] == ["Emb/GatedResidual%s/%s" % (k, leaf) for k in ("", "_1") for leaf in
+                                                  ("entry_offset", "entry_scale", "exit_offset", "exit_scale", "res_scale")]
+    assert len(names) == 10 + 2 * 5
+    for n in names:
+        assert lib._params[n].grad is not None and bool(torch.isfinite(lib._params[n].grad).all()), n
+    with pytest.raises(Exception):
+        slim.gated_res_block(x, activation_fn=torch.sigmoid)
+    # Linear with its input and its activation's mask in 8 bits: same forward, same input gradient
+    xin = torch.randn(70, 40, device=dev)
+    outs = []
+    for save8 in (None, "e4m3"):
+        t = xin.clone().requires_grad_(True)
+        y = lib.ops.linear.Linear("L", 40, 56, t, fused_act="lrelu", save8=save8)
+        dy = torch.randn(70, 56, device=dev, generator=torch.Generator(device=dev).manual_seed(1))
+        W = lib._params["L.W"]
+        outs.append((y.detach(),) + torch.autograd.grad(y, (t, W, lib._params["L.b"]), dy))
+    (y0, dx0, dw0, db0), (y1, dx1, dw1, db1) = outs
+    assert torch.equal(y0, y1) and torch.equal(dx0, dx1)
+    a8 = H.act8_store(xin, "e4m3")
+    dz = H.act_bwd(dy, y0, 2, 0.2)
+    assert torch.equal(dw1, H.linear_wgrad8(a8, dz))
+    mag = dz.abs().sum(0)
+    assert bool(((db0 - db1).abs() <= 2 * R.U * 140 * mag).all())
+    lib.delete_all_params(); slim.reset_scopes()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("mode", ["f32", "bf16"])
+@pytest.mark.parametrize("k,stride,up", [(3, 1, False), (3, 2, False), (1, 1, False), (1, 1, True)])
+def test_conv_layers_with_checkpoints(dev, mode, fmt, k, stride, up):
+    """The layer's output and its input gradient keep every bit; the filter gradient is that of the decoded input."""
+    A, H = _mods()
+    H.set_compute(mode)
+    try:
+        g = torch.Generator().manual_seed(k + stride)
+        dt = BF16 if mode == "bf16" else F32
+        x = torch.relu(torch.randn(2, 8, 12, 64, generator=g)).to(dt).to(dev)
+        w, b = (torch.randn(k, k, 64, 96, generator=g) * 0.05).to(dev), (0.1 * torch.randn(96, generator=g)).to(dev)
+        got = []
+        for f in (None, fmt):
+            A.set_activation_checkpoint(f)
+            leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+            y = A.conv2d(*leaves, stride=stride, act=1, upsample2x=up)
+            assert (y.grad_fn.x8 is not None) == (f is not None)
+            dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(5)).to(y.dtype).to(dev)
+            got.append((y.detach(),) + torch.autograd.grad(y, leaves, dy))
+        A.set_activation_checkpoint(None)
+        (y0, dx0, dw0, db0), (y1, dx1, dw1, db1) = got
+        assert torch.equal(y0, y1) and torch.equal(dx0, dx1)
+        xd = H.act8_load(H.act8_store(x, fmt), dt).requires_grad_(True)
+        leaves = [xd, w.clone().requires_grad_(True), b.clone().requires_grad_(True)]
+        y = A.conv2d(*leaves, stride=stride, act=0, upsample2x=up)
+        dz = H.act_bwd(dy, y0, 1)
+        dwd, = torch.autograd.grad(y, leaves[1:2], dz)
+        # two orders of the same sum of at most 2 * 16 * 24 products: that many roundings of its magnitude (both runs)
+        mag = torch.autograd.grad(A.conv2d(xd.detach().abs(), leaves[1], leaves[2], stride=stride, act=0, upsample2x=up), leaves[1:2], dz.abs())[0]
+        assert bool(((dw1 - dwd).abs() <= 2 * R.U * 800 * mag).all())
+        assert bool(((db1 - db0).abs() <= 2 * R.U * 800 * dz.float().abs().sum((0, 1, 2))).all())
+    finally:
+        H.set_compute("f32")
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("mode", ["f32", "bf16"])
+def test_residual_block_with_checkpoints(dev, mode, fmt):
+    A, H = _mods()
+    H.set_compute(mode)
+    try:
+        g = torch.Generator().manual_seed(7)
+        dt = BF16 if mode == "bf16" else F32
+        x = torch.randn(2, 6, 10, 64, generator=g).to(dt).to(dev)
+        ws = [(torch.randn(3, 3, 64, 64, generator=g) * 0.05).to(dev) for _ in range(2)]
+        bs = [(0.1 * torch.randn(64, generator=g)).to(dev) for _ in range(2)]
+        got = []
+        for f in (None, fmt):
+            A.set_activation_checkpoint(f)
+            leaves = [t.clone().requires_grad_(True) for t in (x, ws[0], bs[0], ws[1], bs[1])]
+            y = A.resblock(*leaves)
+            held = [t for t in y.grad_fn.saved_tensors if t is not None and t.dim() == 4 and t.shape[:3] == x.shape[:3]]
+            assert len(held) == (3 if f is None else 0)
+            dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(5)).to(y.dtype).to(dev)
+            got.append((y.detach(),) + torch.autograd.grad(y, leaves, dy))
+        A.set_activation_checkpoint(None)
+        for k, (p, q) in enumerate(zip(*got)):
+            if k in (2, 4):
+                # filter gradients: the inputs carry the format's rounding, at most 2^-4 (e4m3) or 1 / 64 of the group's largest value
+                # (int8) each; over the 120 terms of random sign 1 / 8 of the largest entry is far out
+                assert float((p - q).abs().max()) <= 0.125 * float(p.abs().max())
+                assert not torch.equal(p, q)
+            else:
+                assert torch.equal(p, q), k
+        with torch.no_grad():
+            A.set_activation_checkpoint(fmt)
+            assert torch.equal(A.resblock(x, ws[0], bs[0], ws[1], bs[1]), got[0][0])
+    finally:
+        H.set_compute("f32")
+
+
+def _step(dev, fmt, mode, graphs):
+    import dpig_amd.tflib as lib
+    from dpig_amd import slim, synthetic
+    from dpig_amd.trainer import Config, DPIG_Encoder_GAN_BodyROI_FgBg
+    lib.delete_all_params(); slim.reset_scopes(); lib.set_device(dev)
+    np.random.seed(1)
+    tr = DPIG_Encoder_GAN_BodyROI_FgBg(Config(batch_size=2, conv_hidden_num=16, z_num=8, act_checkpoint=fmt, compute_dtype=mode), dev)
+    gb = synthetic.to_device(synthetic.make_batch(2, seed=3), dev)
+    tr.init_net(gb)
+    tr.step = 1
+    if graphs:
+        tr.enable_graphs(gb, gb, warmup=1)
+    losses = []
+    for _ in range(3):
+        o = tr.train_step(gb, gb)
+        losses.append((float(o["g_loss"]), float(o["d_loss"])))
+    torch.cuda.synchronize()
+    out = losses, tr.G_flat.flat.detach().clone(), tr.D_flat.flat.detach().clone()
+    lib.delete_all_params(); slim.reset_scopes()
+    return out
+
+
+@pytest.mark.parametrize("mode", ["f32", "bf16"])
+def test_training_steps_with_checkpoints(dev, mode):
+    """Config(act_checkpoint=...): the first step's generator loss is the one without (no forward bit changes), the steps run, and captured steps replay to
+    what eager ones give."""
+    A, H = _mods()
+    try:
+        base, _, _ = _step(dev, None, mode, False)
+        for fmt in ("e4m3", "int8"):
+            losses, G, D = _step(dev, fmt, mode, False)
+            assert losses[0][0] == base[0][0]            # (the critic's loss of the step already sees the updated generator)
+            assert all(np.isfinite(losses).ravel()) and bool(torch.isfinite(G).all()) and bool(torch.isfinite(D).all())
+        again, G2, D2 = _step(dev, "int8", mode, True)
+        assert again == losses and torch.equal(G, G2) and torch.equal(D, D2)
+    finally:
+        H.set_compute("f32")
