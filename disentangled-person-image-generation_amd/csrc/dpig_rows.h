@@ -221,6 +221,19 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
         else if ((C) <= 4096) { CALL(256, 2); }          \
         else { CALL(256, 4); }                           \
     } while (0)
+// ... with one or two vectors per lane up to 4096 channels, for a kernel that holds more values of each
+#define DPIG_ROWS_DISPATCH2(C, CALL)                     \
+    do {                                                 \
+        if ((C) <= 64) { CALL(8, 1); }                   \
+        else if ((C) <= 128) { CALL(16, 1); }            \
+        else if ((C) <= 256) { CALL(32, 1); }            \
+        else if ((C) <= 512) { CALL(64, 1); }            \
+        else if ((C) <= 1024) { CALL(64, 2); }           \
+        else if ((C) <= 2048) { CALL(256, 1); }          \
+        else if ((C) <= 4096) { CALL(256, 2); }          \
+        else { CALL(256, 4); }                           \
+    } while (0)
+inline int lanes_per_row2(int C) { return C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256; }
 inline int lanes_per_row(int C) {
     int lanes = 0;
 #define DPIG_ROWS_LANES(L, N) lanes = L

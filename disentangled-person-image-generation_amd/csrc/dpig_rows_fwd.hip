@@ -1,192 +1,14 @@
-// Norms over the channels of a row, at a residual block's entry and at its exit, forward:
-//   entry  y   = scale * xh + offset,            xh = (x - mean) rstd   (kind 'rms': mean = 0)
-//   exit   out = x + res_scale * gate * (scale * fh + offset),  fh the normed f; optionally the next block's entry norm of `out` (as stored) too
-// and, on request, xh (or fh, or the next norm's xh) as an 8-bit checkpoint from the same registers.
-//
-// Bound by HBM: every operand is read once and every result written once, one wave (or less, or a workgroup) per row with the row in
-// registers; a lane asks for the next row before it works on the present one.  A workgroup takes a contiguous range of rows, so the
-// per-channel operands stay in registers and a gate row is loaded when its group begins.
-#include "dpig_rows.h"
+// The norms' forward kernels on fp32 tensors (dpig_rows_fwd.h), and the C entries of both types.
+#include "dpig_rows_fwd.h"
+
+template <> int dpig::rows::entry_fwd<float>(EntryP p, hipStream_t st) { return entry_fwd_as<float>(p, st); }
+template <> int dpig::rows::exit_fwd<float>(ExitP p, hipStream_t st) { return exit_fwd_as<float>(p, st); }
 
 namespace dpig {
 namespace rows {
 
-struct EntryP {
-    const void* x; void* y;
-    const float *scale, *offset;
-    float *mean, *rstd;
-    long ldx, ldy, nrows, chunk;
-    int C, layer;
-    float eps, rC;
-    Save save;
-};
-
-template <typename T, int LPR, int NV, bool RAG, bool SAVE>
-__global__ __launch_bounds__(NT) void entry_fwd_kernel(const EntryP p) {
-    constexpr int RPB = NT / LPR;
-    __shared__ float red[1][4];
-    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    const long safe = safe_rows(p.nrows, p.C);
-    const T* x = static_cast<const T*>(p.x);
-    T* y = static_cast<T*>(p.y);
-    int n[NV];
-    float sc[NV][8], of[NV][8];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = 8 * (lane + LPR * j);
-        n[j] = p.C - c;
-        ldp(p.scale, c, p.C, 1.f, sc[j]);
-        ldp(p.offset, c, p.C, 0.f, of[j]);
-    }
-    const long r0 = blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.nrows);
-    long r = r0 + sub;
-    Raw8<T> nx[NV];
-    auto fetch = [&](long row) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j], row < safe);
-    };
-    if (r < r1) fetch(r);
-    for (; r < r1; r += RPB) {
-        float v[NV][8];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) unpack(nx[j], v[j]);
-        if (r + RPB < r1) fetch(r + RPB);
-        float mean, rstd;
-        whiten<LPR, NV, RAG>(v, n, (float)p.C, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
-        if (lane == 0) {
-            if (p.mean != nullptr) p.mean[r] = mean;
-            p.rstd[r] = rstd;
-        }
-        if (SAVE) save8<LPR, NV>(p.save, r, lane, v);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], sc[j][e], of[j][e]);
-            st8<RAG>(y + r * p.ldy + 8 * (lane + LPR * j), v[j], n[j]);
-        }
-    }
-}
-
-struct ExitP {
-    const void *x, *f;
-    void *out, *h;                       // h == nullptr: no next norm
-    const float *scale, *offset, *res, *scale2, *offset2;
-    const void* gate;
-    float *mean, *rstd, *mean2, *rstd2;
-    long ldx, ldf, ldo, ldh, nrows, chunk, per;      // per = rows of a gate group
-    int C, layer, layer2, gate_bf16;
-    float eps, eps2, rC;
-    Save save, save2;
-};
-
-// EACH: every row has a gate of its own, fetched with the row; else a gate row is loaded when its group begins
-template <typename T, int LPR, int NV, bool RAG, bool NEXT, bool EACH>
-__global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
-    constexpr int RPB = NT / LPR;
-    __shared__ float red[1][4];
-    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
-    const long safe = safe_rows(p.nrows, p.C);
-    const T *x = static_cast<const T*>(p.x), *f = static_cast<const T*>(p.f);
-    int n[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) n[j] = p.C - 8 * (lane + LPR * j);
-    const long r0 = blockIdx.x * p.chunk, r1 = min(r0 + p.chunk, p.nrows);
-    long r = r0 + sub;
-    Raw8<T> nx[NV], nf[NV];
-    float ng[NV][8];                     // EACH: the next row's gate
-    auto load_gate = [&](long g, int j, float (&m)[8]) {
-        const int c = 8 * (lane + LPR * j);
-        if (p.gate_bf16) ldp(static_cast<const bf16_t*>(p.gate) + g * p.C, c, p.C, 1.f, m);
-        else ldp(static_cast<const float*>(p.gate) + g * p.C, c, p.C, 1.f, m);
-    };
-    auto fetch = [&](long row) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const bool beyond = row < safe;
-            nx[j] = ld8<RAG>(x + row * p.ldx + 8 * (lane + LPR * j), n[j], beyond);
-            nf[j] = ld8<RAG>(f + row * p.ldf + 8 * (lane + LPR * j), n[j], beyond);
-            if (EACH) load_gate(row, j, ng[j]);
-        }
-    };
-    if (r < r1) fetch(r);
-    float a[NV][8], b[NV][8], m[NV][8];  // out = x + m (a fh + b): a, b with the residual scale, m the gate
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = 8 * (lane + LPR * j);
-        float t[8];
-        ldp(p.res, c, p.C, 1.f, t);
-        ldp(p.scale, c, p.C, 1.f, a[j]);
-        ldp(p.offset, c, p.C, 0.f, b[j]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) { a[j][e] *= t[e]; b[j][e] *= t[e]; m[j][e] = 1.f; }
-    }
-    float sc2[NEXT ? NV : 1][8], of2[NEXT ? NV : 1][8];
-    if (NEXT) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            ldp(p.scale2, 8 * (lane + LPR * j), p.C, 1.f, sc2[j]);
-            ldp(p.offset2, 8 * (lane + LPR * j), p.C, 0.f, of2[j]);
-        }
-    }
-    long g = EACH || p.gate == nullptr ? 0 : r / p.per, until = p.gate == nullptr ? p.nrows : (g + 1) * p.per;     // r's group, and its end
-    if (!EACH && p.gate != nullptr && r < r1) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) load_gate(g, j, m[j]);
-    }
-    for (; r < r1; r += RPB) {
-        float v[NV][8], xv[NV][8];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            unpack(nf[j], v[j]);
-            unpack(nx[j], xv[j]);
-            if (EACH) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) m[j][e] = ng[j][e];
-            }
-        }
-        if (r + RPB < r1) fetch(r + RPB);
-        if (!EACH && r >= until) {
-            while (r >= until) { ++g; until += p.per; }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) load_gate(g, j, m[j]);
-        }
-        float mean, rstd;
-        whiten<LPR, NV, RAG>(v, n, (float)p.C, p.rC, p.layer != 0, p.eps, red, &mean, &rstd);
-        if (lane == 0) {
-            if (p.mean != nullptr) p.mean[r] = mean;
-            p.rstd[r] = rstd;
-        }
-        if (p.save.codes != nullptr) save8<LPR, NV>(p.save, r, lane, v);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[j][e] = fmaf(m[j][e], fmaf(v[j][e], a[j][e], b[j][e]), xv[j][e]);
-            st8<RAG>(static_cast<T*>(p.out) + r * p.ldo + 8 * (lane + LPR * j), v[j], n[j]);
-        }
-        if (NEXT) {
-            // the next block's norm sees `out` as it is stored, so that its backward pass can start from the stored tensor
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool in = RAG ? e < n[j] : n[j] > 0;
-                    v[j][e] = in ? round_to(v[j][e], static_cast<T*>(nullptr)) : 0.f;
-                }
-            whiten<LPR, NV, RAG>(v, n, (float)p.C, p.rC, p.layer2 != 0, p.eps2, red, &mean, &rstd);
-            if (lane == 0) {
-                if (p.mean2 != nullptr) p.mean2[r] = mean;
-                p.rstd2[r] = rstd;
-            }
-            if (p.save2.codes != nullptr) save8<LPR, NV>(p.save2, r, lane, v);
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], sc2[j][e], of2[j][e]);
-                st8<RAG>(static_cast<T*>(p.h) + r * p.ldh + 8 * (lane + LPR * j), v[j], n[j]);
-            }
-        }
-    }
-}
+template <> int entry_fwd<bf16_t>(EntryP p, hipStream_t st);      // dpig_rows_fwd_bf16.hip
+template <> int exit_fwd<bf16_t>(ExitP p, hipStream_t st);
 
 // rows per workgroup: a multiple of the rows it takes at a time, about eight workgroups per CU when there are enough rows
 static long fwd_chunk(int64_t nrows, int C) {
@@ -208,42 +30,6 @@ static int check_save(const char* who, int fmt, const uint8_t* codes, const uint
     if (fmt != DPIG_ACT8_E4M3 && fmt != DPIG_ACT8_INT8) return fail(DPIG_EINVAL, "%s: unknown checkpoint format", who);
     if (!aligned16(codes)) return fail(DPIG_EALIGN, "%s: checkpoint codes must be 16-byte aligned", who);
     return DPIG_OK;
-}
-
-template <typename T> static int entry_fwd(EntryP p, hipStream_t st) {
-    const bool rag = p.C % 8 != 0 || !vec_ok(p.x, p.ldx, sizeof(T)) || !vec_ok(p.y, p.ldy, sizeof(T));
-    const bool save = p.save.codes != nullptr;
-    const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
-#define CALL_RS(L, N, R, S) hipLaunchKernelGGL((entry_fwd_kernel<T, L, N, R, S>), grid, dim3(NT), 0, st, p)
-#define CALL(L, N)                                                                                                         \
-    do {                                                                                                                  \
-        if (rag) { if (save) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
-        else { if (save) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
-    } while (0)
-    DPIG_ROWS_DISPATCH(p.C, CALL);
-#undef CALL
-#undef CALL_RS
-    return check_launch("rownorm_fwd");
-}
-template <typename T> static int exit_fwd(ExitP p, hipStream_t st) {
-    const int z = sizeof(T);
-    const bool rag = p.C % 8 != 0 || !vec_ok(p.x, p.ldx, z) || !vec_ok(p.f, p.ldf, z) || !vec_ok(p.out, p.ldo, z) ||
-                     (p.h != nullptr && !vec_ok(p.h, p.ldh, z));
-    const bool next = p.h != nullptr;
-    const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
-    const bool each = p.gate != nullptr && p.per == 1;
-#define CALL_E(L, N, R, S, E) hipLaunchKernelGGL((exit_fwd_kernel<T, L, N, R, S, E>), grid, dim3(NT), 0, st, p)
-#define CALL_RS(L, N, R, S) do { if (each) CALL_E(L, N, R, S, true); else CALL_E(L, N, R, S, false); } while (0)
-#define CALL(L, N)                                                                                                         \
-    do {                                                                                                                  \
-        if (rag) { if (next) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
-        else { if (next) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
-    } while (0)
-    DPIG_ROWS_DISPATCH(p.C, CALL);
-#undef CALL
-#undef CALL_E
-#undef CALL_RS
-    return check_launch("gated_residual_fwd");
 }
 
 }  // namespace rows
