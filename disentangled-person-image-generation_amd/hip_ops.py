@@ -1465,20 +1465,21 @@ def _on_current(device, what):
 def _rows_of(t, what="tensor", like=None):
     """(tensor, rows, C, ld) of an fp32 / bf16 tensor as rows of channels; copied only if its rows are not evenly spaced runs of channels.
     `like`: a tensor whose shape, type and device it has to share."""
-    _require_dev(t)
     if like is None:
+        _require_dev(t)
         _on_current(t.device, what)
-    elif t.shape != like.shape or t.dtype != like.dtype or t.device != like.device:
+    elif t.dtype is not like.dtype or t.shape != like.shape or t.device != like.device:
         raise RuntimeError("%s is %s %s on %s, expected %s %s on %s" % (what, tuple(t.shape), t.dtype, t.device, tuple(like.shape), like.dtype,
                                                                        like.device))
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise RuntimeError("%s has no channels (shape %s)" % (what, tuple(t.shape)))
-    C = t.shape[-1]
+    shape = t.shape
+    C = shape[-1] if len(shape) else 0
+    if C == 0:
+        raise RuntimeError("%s has no channels (shape %s)" % (what, tuple(shape)))
     if t.is_contiguous():
         return t, t.numel() // C, C, C
-    if t.dim() == 2 and (t.stride(1) == 1 or C == 1) and t.stride(0) >= C:
-        return t, t.shape[0], C, t.stride(0)
-    if t.dim() == 4 and t.numel():
+    if len(shape) == 2 and (t.stride(1) == 1 or C == 1) and t.stride(0) >= C:
+        return t, shape[0], C, t.stride(0)
+    if len(shape) == 4 and t.numel():
         ld = nhwc_ld(t)
         if ld is not None:
             return t, t.numel() // C, C, ld
@@ -1487,19 +1488,11 @@ def _rows_of(t, what="tensor", like=None):
 
 
 def _chan(t, C, what, device):
-    """Per-channel fp32 parameter [C] (None passes)."""
+    """fp32 values, one per channel (None passes) or per row."""
     if t is None:
         return None
-    if t.dtype != F32 or t.numel() != C or t.device != device:
+    if t.dtype is not F32 or t.numel() != C or t.device != device:
         raise RuntimeError("%s must be %d fp32 values on %s, got %s %s on %s" % (what, C, device, tuple(t.shape), t.dtype, t.device))
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _row_stat(t, rows, what, device):
-    if t is None:
-        return None
-    if t.dtype != F32 or t.numel() != rows or t.device != device:
-        raise RuntimeError("%s must be %d fp32 values on %s, got %s %s on %s" % (what, rows, device, tuple(t.shape), t.dtype, t.device))
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -1519,6 +1512,11 @@ def _scratch(nbytes, device):
 def _like_rows(t):
     """A contiguous tensor of t's shape and type."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _vectors(n, C, device):
+    """n fp32 [C] tensors of one allocation."""
+    return torch.empty((n, C), dtype=F32, device=device).unbind(0)
 
 
 def act8_store(x, fmt="e4m3"):
@@ -1609,8 +1607,7 @@ def rownorm_fwd(x, scale=None, offset=None, eps=1e-5, kind="layer", save8=None):
     dev = x.device
     scale, offset = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev)
     y = _like_rows(x)
-    mean = torch.empty(rows, dtype=F32, device=dev) if k == 0 else None
-    rstd = torch.empty(rows, dtype=F32, device=dev)
+    mean, rstd = _vectors(2, rows, dev) if k == 0 else (None, torch.empty(rows, dtype=F32, device=dev))
     a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
     if rows:
         check(lib().dpig_rownorm_fwd(ptr(x), int(x.dtype == BF16), ld, rows, C, k, ptr(scale), ptr(offset), eps, ptr(y), C, ptr(mean), ptr(rstd),
@@ -1638,15 +1635,14 @@ def rownorm_bwd(dy, saved, scale, mean, rstd, kind="layer", accum=None, want_par
     dev = dy.device
     scale = _chan(scale, C, "scale", dev)
     xp, ldx, f, codes, scales, keep = _saved_operand(saved, dy, rows)
-    mean, rstd = _row_stat(mean, rows, "mean", dev), _row_stat(rstd, rows, "rstd", dev)
+    mean, rstd = _chan(mean, rows, "mean", dev), _chan(rstd, rows, "rstd", dev)
     if rstd is None or (k == 0 and mean is None and xp is not None):
         raise RuntimeError("rownorm_bwd: the statistics of the forward pass are needed")
     lda = 0
     if accum is not None:
         accum, _, _, lda = _rows_of(accum, "accum", dy)
     dx = _like_rows(dy)
-    dscale = torch.empty(C, dtype=F32, device=dev) if want_params else None
-    doffset = torch.empty(C, dtype=F32, device=dev) if want_params else None
+    dscale, doffset = _vectors(2, C, dev) if want_params else (None, None)
     if rows == 0:
         if want_params:
             dscale.zero_(), doffset.zero_()
@@ -1665,6 +1661,8 @@ def _gate_groups(gate, x, rows, C):
         return None, 0
     if gate.dtype not in (F32, BF16) or gate.device != x.device or gate.dim() == 0 or gate.shape[-1] != C:
         raise RuntimeError("gate must be fp32 or bf16 [..., %d] on %s, got %s %s on %s" % (C, x.device, tuple(gate.shape), gate.dtype, gate.device))
+    if gate.shape == x.shape:
+        return gate.contiguous(), rows
     lead = list(gate.shape[:-1])
     while lead and lead[-1] == 1:
         lead.pop()
@@ -1687,8 +1685,7 @@ def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None,
     scale, offset, res_scale = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev), _chan(res_scale, C, "res_scale", dev)
     gate, groups = _gate_groups(gate, x, rows, C)
     out = _like_rows(x)
-    mean = torch.empty(rows, dtype=F32, device=dev) if k == 0 else None
-    rstd = torch.empty(rows, dtype=F32, device=dev)
+    mean, rstd = _vectors(2, rows, dev) if k == 0 else (None, torch.empty(rows, dtype=F32, device=dev))
     a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
     h = mean2 = rstd2 = a2 = scale2 = offset2 = None
     k2, q2, eps2 = 0, 0, 0.0
@@ -1698,8 +1695,7 @@ def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None,
         q2 = _fmt8(next_save8) if next_save8 is not None else 0
         scale2, offset2 = _chan(scale2, C, "the next norm's scale", dev), _chan(offset2, C, "the next norm's offset", dev)
         h = _like_rows(x)
-        mean2 = torch.empty(rows, dtype=F32, device=dev) if k2 == 0 else None
-        rstd2 = torch.empty(rows, dtype=F32, device=dev)
+        mean2, rstd2 = _vectors(2, rows, dev) if k2 == 0 else (None, torch.empty(rows, dtype=F32, device=dev))
         a2 = _new_act8(x.shape, rows, C, next_save8, dev) if next_save8 is not None else None
     elif next_save8 is not None:
         raise RuntimeError("gated_residual_fwd: next_save8 without next_norm")
@@ -1721,16 +1717,17 @@ def gated_residual_bwd(dout, saved, scale, offset, gate, res_scale, mean, rstd, 
     scale, offset, res_scale = _chan(scale, C, "scale", dev), _chan(offset, C, "offset", dev), _chan(res_scale, C, "res_scale", dev)
     gate, groups = _gate_groups(gate, dout, rows, C)
     fp, ldf, q, codes, scales, keep = _saved_operand(saved, dout, rows)
-    mean, rstd = _row_stat(mean, rows, "mean", dev), _row_stat(rstd, rows, "rstd", dev)
+    mean, rstd = _chan(mean, rows, "mean", dev), _chan(rstd, rows, "rstd", dev)
     if rstd is None or (k == 0 and mean is None and fp is not None):
         raise RuntimeError("gated_residual_bwd: the statistics of the forward pass are needed")
     df = _like_rows(dout)
     dscale = doffset = dgate = dres = None
     if want_params:
-        dscale = torch.empty(C, dtype=F32, device=dev)
-        doffset = torch.empty(C, dtype=F32, device=dev)
+        if res_scale is not None:
+            dscale, doffset, dres = _vectors(3, C, dev)
+        else:
+            dscale, doffset = _vectors(2, C, dev)
         dgate = torch.empty_like(gate) if gate is not None else None
-        dres = torch.empty(C, dtype=F32, device=dev) if res_scale is not None else None
     if rows == 0:
         for t in (dscale, doffset, dgate, dres):
             if t is not None:

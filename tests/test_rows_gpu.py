@@ -310,3 +310,44 @@ def test_two_streams_and_graph_replays(dev, dtype):
             assert all(torch.equal(a, b) for a, b in zip(outs[k], want[k])), rep
         for t in work(*data[rep % 2]):
             float(t.float().sum())
+
+
+def test_rows_beyond_32_bit_offsets(dev):
+    """2^31 elements and more: the last rows are what a small call on them gives, bit for bit."""
+    H = _H()
+    rows, C = 270000, 8192
+    x = torch.empty(rows, C, dtype=BF16, device=dev)
+    x[:16] = 0
+    x[16:] = 1
+    g = torch.Generator(device=dev).manual_seed(1)
+    x[-40:] = torch.randn(40, C, generator=g, device=dev).to(BF16)
+    s, o, r = (_vec(C, i).to(dev) for i in (1, 2, 3))
+    tail = x[-40:].clone()
+    y, mean, rstd, a = H.rownorm_fwd(x, s, o, save8="int8")
+    y2, mean2, rstd2, a2 = H.rownorm_fwd(tail, s, o, save8="int8")
+    assert torch.equal(y[-40:], y2) and torch.equal(rstd[-40:], rstd2) and torch.equal(a.codes[-40:], a2.codes) and torch.equal(a.scales[-40:], a2.scales)
+    assert float(y[:16].float().sub(o).abs().max()) < 0.02 * float(o.abs().max())
+    dx = H.rownorm_bwd(x, a, s, mean, rstd, accum=y, want_params=False)[0]
+    assert torch.equal(dx[-40:], H.rownorm_bwd(tail, a2, s, mean2, rstd2, accum=y2, want_params=False)[0])
+    del dx
+    gate = x[-rows:]
+    out = H.gated_residual_fwd(x, y, s, o, gate, r)[0]
+    assert torch.equal(out[-40:], H.gated_residual_fwd(tail, y2, s, o, tail, r)[0])
+    del out, y
+    q = H.act8_store(x, "e4m3")
+    assert torch.equal(q.codes[-40:], H.act8_store(tail, "e4m3").codes)
+    z = H.act8_load(q, BF16)
+    assert torch.equal(z[-40:], H.act8_load(H.act8_store(tail, "e4m3"), BF16))
+    assert torch.equal(H.act8_act_bwd(x, q, 1)[-40:], torch.where(tail > 0, tail, torch.zeros_like(tail)))
+    # a filter gradient whose dy is a slice of rows 8192 apart; integers, so that every order of the sum is exact
+    del z, q
+    x.copy_(torch.randint(-2, 3, (rows, 1), generator=g, device=dev).to(BF16).expand(rows, C))
+    act = torch.randint(-8, 9, (rows, 40), generator=g, device=dev).float()
+    dw, db = H.linear_wgrad8(H.act8_store(act, "int8"), x[:, 8:24], want_bias=True)
+    assert torch.equal(dw.double(), act.double().t().contiguous() @ x[:, 8:24].double()) and torch.equal(db.double(), x[:, 8:24].double().sum(0))
+
+
+def test_a_tensor_of_another_device_is_refused(dev):
+    H = _H()
+    with pytest.raises(RuntimeError, match="current device"):
+        H._on_current(torch.device("cuda", torch.cuda.current_device() + 1), "x")
