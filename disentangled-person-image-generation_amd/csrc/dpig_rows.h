@@ -203,25 +203,9 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
     }
 }
 
-// Launch shape of a row length: lanes per row and vectors per lane, the smallest that holds it.  The steps of three vectors keep at least two lanes
-// of three at work for every length above 64 (640 channels: 80 of 96 lane-vectors; powers of two alone would give 80 of 128, and took 30 us
-// instead of 24 for the exit's gradient of 32768 rows).
-#define DPIG_ROWS_DISPATCH(C, CALL)                      \
-    do {                                                 \
-        if ((C) <= 64) { CALL(8, 1); }                   \
-        else if ((C) <= 128) { CALL(16, 1); }            \
-        else if ((C) <= 192) { CALL(8, 3); }             \
-        else if ((C) <= 256) { CALL(32, 1); }            \
-        else if ((C) <= 384) { CALL(16, 3); }            \
-        else if ((C) <= 512) { CALL(64, 1); }            \
-        else if ((C) <= 768) { CALL(32, 3); }            \
-        else if ((C) <= 1024) { CALL(64, 2); }           \
-        else if ((C) <= 1536) { CALL(64, 3); }           \
-        else if ((C) <= 2048) { CALL(256, 1); }          \
-        else if ((C) <= 4096) { CALL(256, 2); }          \
-        else { CALL(256, 4); }                           \
-    } while (0)
-// ... with one or two vectors per lane up to 4096 channels, for a kernel that holds more values of each
+// Launch shape of a row length: lanes per row and vectors per lane.  One or two vectors a lane up to 4096 channels; where that leaves a lane in
+// three or more idle (just above a power of two) and there are rows enough for four sets a CU, a quarter of the lanes with three each: 32768 rows of 640
+// channels, the exit's gradient, 24 us instead of 30.  Where the lanes are better filled it does not pay (384 channels: 41.6 against 39.9 us).
 #define DPIG_ROWS_DISPATCH2(C, CALL)                     \
     do {                                                 \
         if ((C) <= 64) { CALL(8, 1); }                   \
@@ -233,13 +217,22 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
         else if ((C) <= 4096) { CALL(256, 2); }          \
         else { CALL(256, 4); }                           \
     } while (0)
+#define DPIG_ROWS_DISPATCH(C, THREE, CALL)               \
+    do {                                                 \
+        if (!(THREE)) DPIG_ROWS_DISPATCH2(C, CALL);      \
+        else if ((C) <= 160) { CALL(8, 3); }             \
+        else if ((C) <= 320) { CALL(16, 3); }            \
+        else if ((C) <= 640) { CALL(32, 3); }            \
+        else { CALL(64, 3); }                            \
+    } while (0)
 inline int lanes_per_row2(int C) { return C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256; }
-inline int lanes_per_row(int C) {
-    int lanes = 0;
-#define DPIG_ROWS_LANES(L, N) lanes = L
-    DPIG_ROWS_DISPATCH(C, DPIG_ROWS_LANES);
-#undef DPIG_ROWS_LANES
-    return lanes;
+inline bool three_vectors(int64_t nrows, int C) {
+    const int lanes = C > 1024 ? 64 : C > 512 ? 32 : C > 256 ? 16 : 8;
+    const bool thin = (C > 128 && C <= 160) || (C > 256 && C <= 320) || (C > 512 && C <= 640) || (C > 1024 && C <= 1280);
+    return thin && nrows * lanes >= 4L * kNumCU * NT;
+}
+inline int lanes_per_row(int64_t nrows, int C) {
+    return !three_vectors(nrows, C) ? lanes_per_row2(C) : C <= 160 ? 8 : C <= 320 ? 16 : C <= 640 ? 32 : 64;
 }
 inline bool vec_ok(const void* p, int64_t ld, int esize) { return aligned16(p) && (ld * esize) % 16 == 0; }
 

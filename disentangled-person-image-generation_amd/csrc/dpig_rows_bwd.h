@@ -303,7 +303,7 @@ template <typename T> inline void launch_rows_as(const BwdP& p, bool groups, uns
         else hipLaunchKernelGGL((rows_bwd_groups_kernel<T, L, N, false>), grid, dim3(NT), 0, st, p);                      \
     } while (0)
     if (groups) DPIG_ROWS_DISPATCH2(p.C, CALL_GROUPS);
-    else DPIG_ROWS_DISPATCH(p.C, CALL);
+    else DPIG_ROWS_DISPATCH(p.C, three_vectors(p.nrows, p.C), CALL);
 #undef CALL
 #undef CALL_GROUPS
 #undef CALL_RS

@@ -137,7 +137,7 @@ static long want_blocks(long sets) {
 static Plan plan(int64_t nrows, int C, bool gated, int64_t groups) {
     Plan q = {};
     const long per = nrows / groups;
-    long rpb = NT / lanes_per_row(C);
+    long rpb = NT / lanes_per_row(nrows, C);
     auto up = [](long a, long b) { return (a + b - 1) / b; };
     if (gated && groups > 1 && per < SHORT_GROUP) {
         q.groups = true;

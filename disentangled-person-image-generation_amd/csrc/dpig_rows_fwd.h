@@ -203,7 +203,7 @@ template <typename T> inline int entry_fwd_as(EntryP p, hipStream_t st) {
         if (rag) { if (save) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
         else { if (save) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
     } while (0)
-    DPIG_ROWS_DISPATCH(p.C, CALL);
+    DPIG_ROWS_DISPATCH(p.C, three_vectors(p.nrows, p.C), CALL);
 #undef CALL
 #undef CALL_RS
     return check_launch("rownorm_fwd");
@@ -222,7 +222,7 @@ template <typename T> inline int exit_fwd_as(ExitP p, hipStream_t st) {
         if (rag) { if (next) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
         else { if (next) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
     } while (0)
-    DPIG_ROWS_DISPATCH(p.C, CALL);
+    DPIG_ROWS_DISPATCH(p.C, three_vectors(p.nrows, p.C), CALL);
 #undef CALL
 #undef CALL_E
 #undef CALL_RS

@@ -12,7 +12,7 @@ template <> int exit_fwd<bf16_t>(ExitP p, hipStream_t st);
 
 // rows per workgroup: a multiple of the rows it takes at a time, about eight workgroups per CU when there are enough rows
 static long fwd_chunk(int64_t nrows, int C) {
-    const long rpb = NT / lanes_per_row(C);
+    const long rpb = NT / lanes_per_row(nrows, C);
     const long want = 8L * kNumCU;
     long it = (nrows + rpb * want - 1) / (rpb * want);
     return (it < 1 ? 1 : it) * rpb;
