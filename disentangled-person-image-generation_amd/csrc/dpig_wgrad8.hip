@@ -66,22 +66,28 @@ __device__ __forceinline__ uint4 to_bf16(const float (&v)[8]) {
     return r.a;
 }
 
-// Behind each of a tile's NM matrix instructions a share of its NL loads
-template <int I, int NM, int NL> __device__ __forceinline__ void weave() {
+// The order of a multiplying phase: behind each of its NM matrix instructions (32 cycles of the matrix pipe) some vector instructions and a share of its
+// NW LDS writes and NL loads
+template <int I, int NM, int NW, int NL> __device__ __forceinline__ void weave() {
     if constexpr (I < NM) {
-        constexpr int l = NL * (I + 1) / NM - NL * I / NM;
+        constexpr int w = NW * (I + 1) / NM - NW * I / NM, l = NL * (I + 1) / NM - NL * I / NM;
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if constexpr (NW > 0) __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+        if constexpr (w > 0) __builtin_amdgcn_sched_group_barrier(0x200, w, 0);
         if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
-        weave<I + 1, NM, NL>();
+        weave<I + 1, NM, NW, NL>();
     }
 }
 
 // Eight waves, WM x 8 / WM, each with MA x NB blocks of 32 x 32; TR rows per tile.
 //
 // A SIMD holds two waves, one of each half of the workgroup, and the halves run half a tile apart: while one multiplies (its fragments in registers, the
-// matrix pipe to itself), the other reads the fragments of its next tile and decodes its share of the tile after that into LDS.  Two barriers a
-// tile keep them apart.  In half-steps h the first half has its memory phase of tile t at h = 2 t and the second at 2 t + 1: tile t + 1 is
-// written at 2 t and 2 t + 1 and read from 2 t + 2 on; its stage held tile t - 1, last read at 2 t - 1.  Two LDS stages do.
+// matrix pipe to itself), the other reads the fragments of its next tile.  Two barriers a tile keep them apart.  In half-steps h the first half reads tile
+// t at h = 2 t and multiplies at 2 t + 1, the second at 2 t + 1 and 2 t + 2.  Where a wave decodes its share of a later tile into LDS:
+//   LATE  between the matrix instructions of its multiplying phase (their 32 cycles leave room).  Tile t + 2 is written at 2 t + 1 and 2 t + 2 and read
+//         from 2 t + 4 on; its stage held tile t - 1, last read at 2 t - 1: three stages.  (65536 x 512 x 512: 46 us, 49 the other way.)
+//   else  behind its reads.  Tile t + 1 is written at 2 t and 2 t + 1 and read from 2 t + 2 on; its stage held tile t - 1: two stages.  The
+//         256 x 256 tile's accumulators leave no registers for more (262144 x 512 x 512: 157 us; 177 with the decoding late, which spills).
 template <typename T, int F, bool RAG, int MA, int NB, int WM, int TR>
 __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
     constexpr bool F32 = sizeof(T) == 4;
@@ -91,7 +97,9 @@ __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
     constexpr int NV = TR / 32, NX = TM / 128, G = TM / 32;             // staging: rows per lane, its pieces of q a row, scales of a row
     constexpr int YC = 16 / (int)sizeof(T), YW = TN / 16 / YC;          // columns of dy a load, loads a row
     constexpr int KS = TR / 16;
-    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+    constexpr bool LATE = MA == 2;                                      // (see above)
+    constexpr int STAGES = LATE ? 3 : 2;
+    __shared__ __attribute__((aligned(16))) char smem[STAGES * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wrow = (wave / WN) * 32 * MA, wcol = (wave % WN) * 32 * NB, l31 = lane & 31, half = lane >> 5;
     const int ntl = p.mtiles * p.ntiles;
@@ -288,29 +296,34 @@ __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
     };
     Regs g[2];
     const int ntr = (have_rows + TR - 1) / TR;
+    int byte[NV];
     fetch(g[0]);
     fetch(g[1]);
-    int byte[NV];
-    bias_turn(g[0]);
-    scales(g[0], byte);
-    stage(g[0], byte, smem);
-    fetch(g[0]);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {                // tiles 0 (and 1) into LDS, the two after them on their way
+        bias_turn(g[i]);
+        scales(g[i], byte);
+        stage(g[i], byte, smem + i * STAGE);
+        fetch(g[i]);
+    }
     barrier();
     if (wave >= 4) barrier();                             // the second half: half a tile behind
     int t = 0;
     auto step = [&](auto I) {
-        constexpr int i = decltype(I)::value;             // t % 2
-        constexpr int NM = KS * TERMS * MA * NB, NL = NV * (NX + YW) + 1;
-        Regs& s = g[i ^ 1];                               // tile t + 1
+        constexpr int i = decltype(I)::value;             // t % 6
+        constexpr int NM = KS * TERMS * MA * NB, NW = LATE ? NV * (NX + YW * TERMS) : 0, NL = NV * (NX + YW) + 1;
+        constexpr int later = (i + STAGES - 1) % STAGES;  // the stage of tile t + STAGES - 1
+        Regs& s = g[(i + STAGES - 1) & 1];                // that tile
         scales(s, byte);
-        read(smem + i * STAGE);
-        stage(s, byte, smem + (i ^ 1) * STAGE);
+        read(smem + i % STAGES * STAGE);
+        if (!LATE) stage(s, byte, smem + later * STAGE);
         bias_turn(s);
         barrier();
         __builtin_amdgcn_s_setprio(1);
-        fetch(s);                                         // tile t + 3
+        if (LATE) stage(s, byte, smem + later * STAGE);
+        fetch(s);                                         // two tiles further on
         multiply();
-        weave<0, NM, NL>();
+        weave<0, NM, NW, NL>();
         __builtin_amdgcn_s_setprio(0);
         barrier();
         return ++t < ntr;
@@ -318,6 +331,12 @@ __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
     for (;;) {
         if (!step(std::integral_constant<int, 0>())) break;
         if (!step(std::integral_constant<int, 1>())) break;
+        if constexpr (LATE) {
+            if (!step(std::integral_constant<int, 2>())) break;
+            if (!step(std::integral_constant<int, 3>())) break;
+            if (!step(std::integral_constant<int, 4>())) break;
+            if (!step(std::integral_constant<int, 5>())) break;
+        }
     }
     if (wave < 4) barrier();
 
@@ -342,16 +361,16 @@ __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
             }
     }
     if (p.want_db && (p.nsplit > 1 || mt == 0)) {     // workgroup-uniform; the staging buffers are free
-        float(*bs)[TN] = reinterpret_cast<float(*)[TN]>(smem);       // [32 rows][TN columns]
+        float(*sums)[TN] = reinterpret_cast<float(*)[TN]>(smem);     // [32 rows][TN columns]
 #pragma unroll
         for (int w = 0; w < YW; ++w)
 #pragma unroll
-            for (int e = 0; e < YC; ++e) bs[wave * 4 + sr][(16 * w + sg) * YC + e] = bias[w][e];
+            for (int e = 0; e < YC; ++e) sums[wave * 4 + sr][(16 * w + sg) * YC + e] = bias[w][e];
         __syncthreads();
         if (tid < TN && k0 + tid < p.K) {
             float s = 0.f;
 #pragma unroll 8
-            for (int r = 0; r < 32; ++r) s += bs[r][tid];
+            for (int r = 0; r < 32; ++r) s += sums[r][tid];
             if (p.bias_partial) p.bias_partial[((long)split * (p.nsplit > 1 ? p.mtiles : 1) + mt) * p.K + k0 + tid] = s;
             else p.db[k0 + tid] = p.beta_b != 0.f ? p.beta_b * p.db[k0 + tid] + s : s;
         }
