@@ -188,9 +188,10 @@ def test_linear_wgrad8_reads_every_value_exactly(dev, rows, C, dtype, fmt):
     assert torch.equal(db.cpu(), torch.ones(rows))
 
 
-# the 256 x 128 and 256 x 256 tiles are taken from 2^32 and 2^35 products on (fp32 dy: a third of that)
+# the 256 x 128 and 256 x 256 tiles are taken above 10^10 and 2^35 products (fp32 dy: a third of that)
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
-@pytest.mark.parametrize("rows,C,K,dtype", [(33000, 250, 520, BF16), (133001, 500, 520, BF16), (133001, 512, 513, BF16), (40001, 200, 260, F32)])
+@pytest.mark.parametrize("rows,C,K,dtype", [(90001, 250, 520, BF16), (90001, 250, 519, BF16), (140001, 500, 520, BF16), (140001, 512, 513, BF16),
+                                              (80001, 200, 260, F32)])
 def test_linear_wgrad8_large_tiles_are_exact_on_integers(dev, rows, C, K, dtype, fmt):
     H = _H()
     g = torch.Generator(device=dev).manual_seed(rows)
