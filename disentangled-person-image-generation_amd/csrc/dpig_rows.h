@@ -127,14 +127,15 @@ template <int LPR, int NS> __device__ __forceinline__ void row_sums(float (&s)[N
 // s / C and 1 / sqrt(a), each within about half a step: the scale of a whole row hangs on them, and with it the side on which every value of the
 // row falls when it is rounded to 8 bits
 __device__ __forceinline__ float over_count(float s, float C, float rC) {
-    const float q = s * rC;
-    return fmaf(fmaf(-q, C, s), rC, q);
+    const float q = s * rC, f = fmaf(fmaf(-q, C, s), rC, q);
+    return f == f ? f : q;                                    // (a sum that overflowed stays infinite)
 }
 __device__ __forceinline__ float inv_sqrt(float a) {
     const float r = __builtin_amdgcn_rsqf(a);
     const float h = a * r, l = fmaf(a, r, -h);
     const float e = fmaf(-l, r, fmaf(-h, r, 1.f));           // 1 - a r r
-    return fmaf(0.5f * r, e, r);
+    const float f = fmaf(0.5f * r, e, r);
+    return f == f ? f : r;                                    // (1 / sqrt of infinity is zero, of zero infinite)
 }
 
 // Statistics of a row held in registers, and the row normed in place: mean first, then the sum of squares about it (no cancellation).

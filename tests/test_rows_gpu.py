@@ -244,6 +244,12 @@ def test_values_that_are_not_finite_stay_in_their_rows(dev):
     bad = torch.isnan(y).all(1).cpu().nonzero().flatten().tolist()
     assert bad == [3, 9, 20] and bool(torch.isfinite(y.cpu()[[i for i in range(40) if i not in bad]]).all())
     assert (a.scales.cpu() == 255).all(1).nonzero().flatten().tolist() == bad
+    big = torch.full((3, 96), 1e25)                                       # squares beyond fp32: rstd = 0, and with it xh
+    big[:, ::2] *= -1
+    big[1] = torch.randn(96, generator=torch.Generator().manual_seed(3))
+    for kind in ("layer", "rms"):
+        y, _, rstd, _ = H.rownorm_fwd(big.to(dev), None, None, EPS, kind, save8="int8")
+        assert rstd.cpu()[[0, 2]].tolist() == [0.0, 0.0] and float(y[[0, 2]].abs().sum()) == 0.0 and float(y[1].abs().max()) > 1
     z = torch.zeros(4, 96, device=dev)                                    # a row of zeros: xh = 0, not NaN
     y, _, rstd, _ = H.rownorm_fwd(z, None, None, EPS, "rms")
     assert float(y.abs().sum()) == 0.0 and bool(torch.isfinite(rstd).all())
@@ -351,3 +357,60 @@ def test_a_tensor_of_another_device_is_refused(dev):
     H = _H()
     with pytest.raises(RuntimeError, match="current device"):
         H._on_current(torch.device("cuda", torch.cuda.current_device() + 1), "x")
+
+
+@pytest.mark.parametrize("rows,C,groups", [(96, 200, 4), (640, 64, 20), (40, 130, 20), (33 * 64, 96, 64)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_bf16_gates(dev, rows, C, groups, dtype):
+    """A bf16 gate per group, in every form: what the same gate in fp32 gives; its gradient is that one rounded."""
+    H = _H()
+    x, f, dy = (_rand(rows, C, i, dtype).to(dev) for i in (1, 2, 3))
+    s, o, r = (_vec(C, i).to(dev) for i in (1, 2, 3))
+    gate = _rand(groups, C, 4, BF16).to(dev)
+    a, b = H.gated_residual_fwd(x, f, s, o, gate, r), H.gated_residual_fwd(x, f, s, o, gate.float(), r)
+    assert torch.equal(a[0], b[0])
+    p, q = (H.gated_residual_bwd(dy, f, s, o, g, r, a[1], a[2]) for g in (gate, gate.float()))
+    assert p[3].dtype == BF16 and torch.equal(p[3], q[3].to(BF16))
+    for k in (0, 1, 2, 4):
+        assert torch.equal(p[k], q[k])
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("C,ld", [(64, 80), (37, 45), (250, 256)])
+def test_strided_results_leave_what_lies_between_their_rows(dev, bf16, C, ld):
+    """The C entries with row strides of their own: nothing is written between the rows, before the first or behind the last."""
+    from dpig_amd import _lib
+    h, rows, dt = _lib.lib(), 70, BF16 if bf16 else F32
+    st = _lib.stream_ptr()
+
+    def field():
+        return torch.full((rows + 2, ld), 7.0, dtype=dt, device=dev)
+
+    def inside(t):
+        return t.view(-1)[ld + 3:].as_strided((rows, C), (ld, 1))
+
+    def check(t, want):
+        assert torch.equal(inside(t), want)
+        inside(t).fill_(7.0)
+        assert bool((t == 7.0).all())
+    H = _H()
+    x, f, dy = (_rand(rows, C, i, dt).to(dev) for i in (1, 2, 3))
+    s, o = _vec(C, 1).to(dev), _vec(C, 2).to(dev)
+    m, r, m2, r2 = torch.empty(4, rows, device=dev).unbind(0)
+    P = lambda t: t.data_ptr()      # noqa: E731
+    y, hh = field(), field()
+    assert h.dpig_rownorm_fwd(P(x), bf16, C, rows, C, 0, P(s), P(o), EPS, P(inside(y)), ld, P(m), P(r), 0, None, None, st) == 0
+    check(y, H.rownorm_fwd(x, s, o)[0])
+    assert h.dpig_gated_residual_fwd(P(x), C, P(f), C, bf16, rows, C, 0, P(s), P(o), EPS, None, 0, 0, None, P(inside(y)), ld, P(m), P(r), 0, None, None,
+                                     0, P(s), P(o), EPS, P(inside(hh)), ld, P(m2), P(r2), 0, None, None, st) == 0
+    out, mean, rstd, _, after = H.gated_residual_fwd(x, f, s, o, next_norm=(s, o, EPS, "layer"))
+    check(y, out)
+    check(hh, after[0])
+    assert h.dpig_gated_residual_bwd(P(dy), bf16, C, P(f), C, 0, None, None, rows, C, 0, P(s), P(o), None, 0, 0, None, P(mean), P(rstd), P(inside(y)), ld,
+                                     None, None, None, None, None, 0, st) == 0
+    check(y, H.gated_residual_bwd(dy, f, s, o, None, None, mean, rstd, want_params=False)[0])
+    a = H.act8_store(x, "int8")
+    assert h.dpig_act8_load(P(a.codes), P(a.scales), rows, C, 1, P(inside(y)), bf16, ld, st) == 0
+    check(y, H.act8_load(a, dt))
+    assert h.dpig_act8_act_bwd(P(dy), bf16, C, P(a.codes), rows, C, 1, 2, 0.2, P(inside(y)), ld, st) == 0
+    check(y, H.act8_act_bwd(dy, a, 2))
