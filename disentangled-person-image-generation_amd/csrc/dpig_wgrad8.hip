@@ -4,8 +4,8 @@
 // norm's xh serves both the norm's gradient and this product, and the scale / offset cost one multiply-add per element of dw.
 //
 // Products on the bf16 matrix pipe, accumulation in fp32.  q is exact in bf16 (dpig_act8.h).  A bf16 dy is used as it is; an fp32 dy is cut
-// into three bf16 terms (8 + 8 + 8 significand bits) whose products are exact in fp32, so the result is that of fp32 products -- at three of the bf16
-// pipe's MFMAs, 16 / 3 times the fp32 pipe's rate.
+// into three bf16 terms (8 + 8 + 8 significand bits, each the rest's leading ones) whose products are exact in fp32, so the result is that of fp32
+// products -- at three of the bf16 pipe's MFMAs, 16 / 3 times the fp32 pipe's rate.  (An infinite dy leaves a rest that is not a number: NaN.)
 //
 // GEMM rows = c (128 per workgroup), columns = k (128), reduction = rows r (TR per tile).  Both operands lie reduction-major in HBM while an
 // MFMA lane wants 8 consecutive r of one column: tiles are staged [r][128 columns] as bf16 (codes are decoded, fp32 gradients cut, on their
@@ -60,12 +60,6 @@ template <int F> __device__ __forceinline__ uint4 decode_bf16(unsigned q0, unsig
     }
     return r;
 }
-__device__ __forceinline__ uint4 to_bf16(const float (&v)[8]) {
-    Raw8<bf16_t> r;
-    pack(v, r);
-    return r.a;
-}
-
 // The order of a multiplying phase: behind each of its NM matrix instructions (32 cycles of the matrix pipe) some vector instructions and a share of its
 // NW LDS writes and NL loads
 template <int I, int NM, int NW, int NL> __device__ __forceinline__ void weave() {
@@ -197,14 +191,16 @@ __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
                 if constexpr (!F32) {
                     *reinterpret_cast<u32x4*>(yt + r * YROW + (((16 * w + sg) ^ swz) << 4)) = g.yv[i][w];
                 } else {
+                    // the upper halves of fp32 values are their first eight significand bits in bf16; what is left has the next sixteen
                     float v[4];
                     widen(g.yv[i][w], v);
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t) {
-                        const unsigned a = (unsigned)f2bf(v[0]) | ((unsigned)f2bf(v[1]) << 16), b = (unsigned)f2bf(v[2]) | ((unsigned)f2bf(v[3]) << 16);
-                        *reinterpret_cast<uint2*>(yt + t * YTILE + r * YROW + (((8 * w + (sg >> 1)) ^ swz) << 4) + 8 * (sg & 1)) = make_uint2(a, b);
-                        v[0] -= __uint_as_float(a << 16); v[1] -= __uint_as_float(a & 0xffff0000u);      // exact: the rest of a rounding
-                        v[2] -= __uint_as_float(b << 16); v[3] -= __uint_as_float(b & 0xffff0000u);
+                        const u32x2 h = {__builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u),
+                                         __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u)};
+                        *reinterpret_cast<u32x2*>(yt + t * YTILE + r * YROW + (((8 * w + (sg >> 1)) ^ swz) << 4) + 8 * (sg & 1)) = h;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] -= __uint_as_float(__float_as_uint(v[e]) & 0xffff0000u);
                     }
                 }
             }

@@ -202,18 +202,33 @@ def test_linear_wgrad8_large_tiles_are_exact_on_integers(dev, rows, C, K, dtype,
     assert torch.equal(dw.double(), want) and torch.equal(db.double(), dy.double().sum(0))
 
 
-def test_linear_wgrad8_strides_and_not_finite_values(dev):
+@pytest.mark.parametrize("rows", [40, 3000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_wgrad8_adds_into_given_buffers(dev, rows, dtype):
+    """beta and db_beta without an affine part, written in place (few rows) and joined (many)."""
     H = _H()
-    x, dy, _, _ = _operands(300, 70, 90, F32, "e4m3", 9)
+    g = torch.Generator().manual_seed(rows)
+    q, dy = torch.randint(-9, 10, (rows, 70), generator=g), torch.randint(-3, 4, (rows, 50), generator=g)
+    out, db = torch.full((70, 50), 2.0, device=dev), torch.full((50,), 3.0, device=dev)
+    H.linear_wgrad8(H.act8_store(q.float().to(dev), "int8"), dy.to(dtype).to(dev), out=out, beta=0.5, db=db, db_beta=2.0)
+    assert torch.equal(out.double().cpu(), q.double().t() @ dy.double() + 1) and torch.equal(db.double().cpu(), dy.double().sum(0) + 6)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_linear_wgrad8_strides_and_not_finite_values(dev, fmt):
+    H = _H()
+    x, dy, _, _ = _operands(300, 70, 90, F32, fmt, 9)
+    big = H.linear_wgrad8(H.act8_store(x.to(dev), fmt), torch.full((300, 4), 3.4e38, device=dev) * torch.tensor([1.0, -1.0, 0.0, 1e-30], device=dev))
+    assert bool(torch.isfinite(big[:, 2:]).all()) and not bool(torch.isnan(big).any())       # (finite, however large: no NaN)
     x[11, 40] = float("inf")
     wide = torch.randn(300, 128)
     wide[:, 3:93] = dy
-    a = H.act8_store(x.to(dev), "e4m3")
+    a = H.act8_store(x.to(dev), fmt)
     dw = H.linear_wgrad8(a, wide.to(dev)[:, 3:93])
     bad = torch.isnan(dw).all(1).cpu()
     assert bad.nonzero().flatten().tolist() == list(range(32, 64))        # the group that held the infinity, and nothing else
     x[11, 40] = 0
-    ref = H.linear_wgrad8(H.act8_store(x.to(dev), "e4m3"), dy.to(dev))
+    ref = H.linear_wgrad8(H.act8_store(x.to(dev), fmt), dy.to(dev))
     keep = ~bad
     assert torch.equal(dw.cpu()[keep], ref.cpu()[keep])
     d4 = torch.randn(4, 5, 15, 90)                                       # channel-last maps: rows are the pixels
