@@ -192,7 +192,7 @@ def test_conv_layers_with_checkpoints(dev, mode, fmt, k, stride, up):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
-@pytest.mark.parametrize("mode", ["f32", "bf16"])
+@pytest.mark.parametrize("mode", ["f32", "bf16", "f32w", "bf16x3"])
 def test_residual_block_with_checkpoints(dev, mode, fmt):
     A, H = _mods()
     H.set_compute(mode)
