@@ -322,7 +322,9 @@ def _sink_small(p, g):
 
 # ---- activations kept for the backward pass in 8 bits ---------------------------------------------------------------------------
 # With a format set, the conv / residual block / fully connected Functions keep hip_ops.Act8 checkpoints of their inputs and activation outputs
-# instead of the tensors: 33/32 bytes an element against 2 or 4 (a quarter of fp32's, half of bf16's where nobody else holds the tensor).
+# instead of the tensors: 33/32 bytes an element against 4 or 2.  (An activation's output that feeds another layer is kept by both, each its own.)
+# The 16-image 128 x 64 training step holds 1.60 GB beyond its parameters instead of 3.33 in 'f32w', 39.3 ms instead of 37.8, and 1.24 GB instead
+# of 1.68 in 'bf16', 16.4 ms instead of 14.3 (both uncaptured).
 # The backward pass reads them: activation masks and the filter gradients of 1x1 / fully connected layers directly, other filter gradients from
 # values decoded into a scratch tensor.  Forward results are unchanged; filter gradients see inputs rounded to 8 bits.
 SAVE8 = [None]
@@ -339,8 +341,8 @@ class _Kept8(object):
     """A checkpoint with the type of the tensor it stands for."""
     __slots__ = ("a", "dtype")
 
-    def __init__(self, t, fmt):
-        self.a, self.dtype = H.act8_store(t, fmt), t.dtype
+    def __init__(self, a, dtype):
+        self.a, self.dtype = a, dtype
 
     @property
     def shape(self):
@@ -367,8 +369,24 @@ def _worth8(t, fmt):
 
 
 def _keep(t, fmt):
-    """(tensor to save, checkpoint): one of the two is None."""
-    return (None, _Kept8(t, fmt)) if _worth8(t, fmt) else (t, None)
+    """(tensor to save, its Act8): one of the two is None."""
+    return (None, H.act8_store(t, fmt)) if _worth8(t, fmt) else (t, None)
+
+
+def _save(ctx, tensors, *acts):
+    """save_for_backward with checkpoints: pairs of an Act8 (or None) and the type of the tensor it stands for.  Codes and scales are saved tensors like
+    others, freed by the backward pass as it goes."""
+    ctx.meta8 = [None if a is None else (a.shape, a.fmt, dtype) for a, dtype in acts]
+    flat = [t for a, _ in acts for t in ((None, None) if a is None else (a.codes, a.scales))]
+    ctx.save_for_backward(*tensors, *flat)
+
+
+def _saved(ctx):
+    """(tensors, checkpoints as _Kept8 or None) that `_save` got."""
+    t, n = ctx.saved_tensors, len(ctx.meta8)
+    flat = t[len(t) - 2 * n:]
+    return t[:len(t) - 2 * n], [None if m is None else _Kept8(H.Act8(flat[2 * k], flat[2 * k + 1], m[0], m[1]), m[2])
+                                for k, m in enumerate(ctx.meta8)]
 
 
 def _sink_wgrad8(w, b, a, dz, want_w, want_b, scale=None, offset=None):
@@ -491,18 +509,18 @@ class _ConvFn(torch.autograd.Function):
         else:
             y = H.conv2d_fwd(x, w, b, stride=stride, act=act, alpha=alpha, upsample2x=upsample2x,
                              out=out.t if out is not None else None, emit32=True)      # (a conv's output mostly feeds a conv)
-        ctx.x_shape = tuple(x.shape)
-        x, ctx.x8 = _keep(x, save8)
-        y_kept, ctx.y8 = _keep(y, save8) if act != ACT_NONE else (None, None)
-        ctx.save_for_backward(x, w, y_kept)
+        ctx.x_shape, dtype = tuple(x.shape), x.dtype
+        x, x8 = _keep(x, save8)
+        y_kept, y8 = _keep(y, save8) if act != ACT_NONE else (None, None)
+        _save(ctx, (x, w, y_kept), (x8, dtype), (y8, y.dtype))
         ctx.cfg = (stride, act, alpha, upsample2x, b is not None)
         ctx.b_ref = b
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, w, y = ctx.saved_tensors
-        x8, y8, x_shape = ctx.x8, ctx.y8, ctx.x_shape
+        (x, w, y), (x8, y8) = _saved(ctx)
+        x_shape = ctx.x_shape
         stride, act, alpha, up, has_b = ctx.cfg
         second = torch.is_grad_enabled()       # backward under create_graph=True
         if y8 is not None and (second or up):
@@ -573,34 +591,32 @@ class _ResBlockFn(torch.autograd.Function):
         c2 = torch.empty_like(c1)
         out = torch.empty_like(c1) if out is None else out.t
         H.conv2d_fwd(c1, w2, b2, act=ACT_RELU, residual=x0, res_after_act=True, out=out, out_act=c2, emit32=True)
-        ctx.k8 = None
         if _worth8(x0, save8):
-            ctx.k8 = tuple(_Kept8(t, save8) for t in (x0, c1, c2))
-            ctx.save_for_backward(None, w1, w2, None, None)
+            _save(ctx, (None, w1, w2, None, None), *((H.act8_store(t, save8), t.dtype) for t in (x0, c1, c2)))
         else:
-            ctx.save_for_backward(x0, w1, w2, c1, c2)
+            _save(ctx, (x0, w1, w2, c1, c2))
         ctx.b_refs = (b1, b2)
         return out
 
     @staticmethod
     def backward(ctx, dout):
-        x0, w1, w2, c1, c2 = ctx.saved_tensors
+        (x0, w1, w2, c1, c2), k8 = _saved(ctx)
         b1, b2 = ctx.b_refs
-        if ctx.k8 is not None:
-            x8, c18, c28 = ctx.k8
+        if k8:
+            x8, c18, c28 = k8
             dz2 = c28.act_bwd(dout, ACT_RELU)
             c1 = c18.load()                         # (values for the filter gradient, signs for the mask)
         else:
             dz2 = H.act_bwd(dout, c2, ACT_RELU, emit32=True)
         dw2, db2 = _sink_wgrad_bias(w2, b2, c1, dz2, want_w=ctx.needs_input_grad[3], want_b=ctx.needs_input_grad[4])
         dz1 = H.conv2d_dgrad(dz2, w2, tuple(c1.shape), mask=c1, act=ACT_RELU, emit32=True)    # feeds dgrad(conv1)
-        if ctx.k8 is not None:
+        if k8:
             del c1
             x0 = x8.load()
         dw1, db1 = _sink_wgrad_bias(w1, b1, x0, dz1, want_w=ctx.needs_input_grad[1], want_b=ctx.needs_input_grad[2])
         dx0 = None
         if ctx.needs_input_grad[0]:
-            if ctx.x0_relu and FUSE_INPUT_MASK[0] and not torch.is_grad_enabled() and ctx.k8 is None:
+            if ctx.x0_relu and FUSE_INPUT_MASK[0] and not torch.is_grad_enabled() and not k8:
                 # x0 is a ReLU conv's output: hand its producer the gradient w.r.t. the PRE-activation (mask in this epilogue)
                 dx0 = H.conv2d_dgrad(dz1, w1, tuple(x0.shape), accum=dout, mask=x0, act=ACT_RELU)
                 dx0._dpig_masked_for = (x0.data_ptr(), dx0._version)
@@ -888,34 +904,34 @@ class _LinearFn(torch.autograd.Function):
     def forward(ctx, x, w, b, act, alpha, save8=None):
         y = H.linear_fwd(x, w, b, act=act, alpha=alpha)
         ctx.x_dtype = x.dtype
-        x, ctx.x8 = _keep(x, save8)
-        y_kept, ctx.y8 = _keep(y, save8) if act != ACT_NONE else (None, None)
-        ctx.save_for_backward(x, w, y_kept)
+        x, x8 = _keep(x, save8)
+        y_kept, y8 = _keep(y, save8) if act != ACT_NONE else (None, None)
+        _save(ctx, (x, w, y_kept), (x8, ctx.x_dtype), (y8, y.dtype))
         ctx.cfg = (act, alpha, b is not None)
         ctx.b_ref = b
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, w, y = ctx.saved_tensors
+        (x, w, y), (x8, y8) = _saved(ctx)
         act, alpha, has_b = ctx.cfg
         if torch.is_grad_enabled():            # backward under create_graph=True
-            if ctx.y8 is not None:
-                y = ctx.y8.load()
+            if y8 is not None:
+                y = y8.load()
             dz = _ActBwdFn.apply(dy, y, act, alpha) if act != ACT_NONE else dy.contiguous()
             dx = _LinearDgradFn.apply(dz, w) if ctx.needs_input_grad[0] else None
             dz = dz.detach()
         else:
-            if ctx.y8 is not None:
-                dz = ctx.y8.act_bwd(dy, act, alpha)
+            if y8 is not None:
+                dz = y8.act_bwd(dy, act, alpha)
             else:
                 dz = H.act_bwd(dy, y, act, alpha) if act != ACT_NONE else dy.contiguous()
             dx = H.linear_dgrad(dz, w) if ctx.needs_input_grad[0] else None
         dw = db = None
         want_w = ctx.needs_input_grad[1] and not _PARAM_GRADS_OFF[0]
         want_b = has_b and ctx.needs_input_grad[2] and not _PARAM_GRADS_OFF[0]
-        if ctx.x8 is not None:
-            dw, db = _sink_wgrad8(w, ctx.b_ref, ctx.x8.a, dz, want_w, want_b)
+        if x8 is not None:
+            dw, db = _sink_wgrad8(w, ctx.b_ref, x8.a, dz, want_w, want_b)
         else:
             if want_w:
                 dw = _sink(w, lambda o, beta: H.linear_wgrad(x, dz, out=o, beta=beta))
@@ -939,17 +955,17 @@ class _RowNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, scale, offset, eps, kind, save8):
         y, mean, rstd, a = H.rownorm_fwd(x, scale, offset, eps, kind, save8=save8)
-        ctx.a, ctx.kind, ctx.offset_ref = a, kind, offset
-        ctx.save_for_backward(None if a is not None else x, scale, mean, rstd)
+        ctx.kind, ctx.offset_ref = kind, offset
+        _save(ctx, (None if a is not None else x, scale, mean, rstd), (a, x.dtype))
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, scale, mean, rstd = ctx.saved_tensors
+        (x, scale, mean, rstd), (x8,) = _saved(ctx)
         off = _PARAM_GRADS_OFF[0]
         want_s, want_o = ctx.needs_input_grad[1] and not off, ctx.needs_input_grad[2] and not off
-        dx, ds, do = H.rownorm_bwd(dy, ctx.a if x is None else x, scale, mean, rstd, ctx.kind, want_params=want_s or want_o)
+        dx, ds, do = H.rownorm_bwd(dy, x8.a if x is None else x, scale, mean, rstd, ctx.kind, want_params=want_s or want_o)
         return (dx, _sink_small(scale, ds) if want_s else None, _sink_small(ctx.offset_ref, do) if want_o else None, None, None, None)
 
 
@@ -963,18 +979,18 @@ class _GatedResidualFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, scale, offset, gate, res_scale, eps, kind, save8):
         out, mean, rstd, a, _ = H.gated_residual_fwd(x, f, scale, offset, gate, res_scale, eps, kind, save8=save8)
-        ctx.a, ctx.kind = a, kind
+        ctx.kind = kind
         ctx.refs = (scale, offset, res_scale)
-        ctx.save_for_backward(None if a is not None else f, scale, offset, gate, res_scale, mean, rstd)
+        _save(ctx, (None if a is not None else f, scale, offset, gate, res_scale, mean, rstd), (a, f.dtype))
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        f, scale, offset, gate, res_scale, mean, rstd = ctx.saved_tensors
+        (f, scale, offset, gate, res_scale, mean, rstd), (f8,) = _saved(ctx)
         need, off = ctx.needs_input_grad, _PARAM_GRADS_OFF[0]
         want = need[4] or (not off and (need[2] or need[3] or need[5]))
-        df, ds, do, dg, dr = H.gated_residual_bwd(dout, ctx.a if f is None else f, scale, offset, gate, res_scale, mean, rstd, ctx.kind, want_params=want)
+        df, ds, do, dg, dr = H.gated_residual_bwd(dout, f8.a if f is None else f, scale, offset, gate, res_scale, mean, rstd, ctx.kind, want_params=want)
         sink = [_sink_small(p, g) if n and not off else None for p, g, n in zip(ctx.refs, (ds, do, dr), (need[2], need[3], need[5]))]
         return (dout if need[0] else None, df if need[1] else None, sink[0], sink[1], dg.view(gate.shape) if need[4] else None, sink[2],
                 None, None, None)
@@ -1000,9 +1016,8 @@ class _GatedBlockFn(torch.autograd.Function):
         f = H.linear_fwd(u, w2, b2)
         f = (H.to_bf16(f) if x.dtype == H.BF16 else f).view(x.shape)
         out, m2, r2, f8, _ = H.gated_residual_fwd(x, f, s2, o2, gate, res_scale, eps, kind, save8=save8)
-        ctx.kept8 = (x8, u8, f8)
         keep = (None, None, None, None) if save8 is not None else (x, h, u, f)
-        ctx.save_for_backward(*keep, s1, o1, w1, w2, s2, o2, gate, res_scale, m1, r1, m2, r2)
+        _save(ctx, (*keep, s1, o1, w1, w2, s2, o2, gate, res_scale, m1, r1, m2, r2), (x8, x.dtype), (u8, u.dtype), (f8, f.dtype))
         ctx.refs = (s1, o1, b1, b2, s2, o2, res_scale)
         ctx.cfg = (act, alpha, kind)
         return out
@@ -1010,8 +1025,8 @@ class _GatedBlockFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        x, h, u, f, s1, o1, w1, w2, s2, o2, gate, res_scale, m1, r1, m2, r2 = ctx.saved_tensors
-        x8, u8, f8 = ctx.kept8
+        (x, h, u, f, s1, o1, w1, w2, s2, o2, gate, res_scale, m1, r1, m2, r2), kept = _saved(ctx)
+        x8, u8, f8 = (k.a if k is not None else None for k in kept)
         rs1, ro1, b1, b2, rs2, ro2, rres = ctx.refs
         act, alpha, kind = ctx.cfg
         off = _PARAM_GRADS_OFF[0]

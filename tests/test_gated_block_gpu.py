@@ -172,7 +172,7 @@ def test_conv_layers_with_checkpoints(dev, mode, fmt, k, stride, up):
             A.set_activation_checkpoint(f)
             leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
             y = A.conv2d(*leaves, stride=stride, act=1, upsample2x=up)
-            assert (y.grad_fn.x8 is not None) == (f is not None)
+            assert (y.grad_fn.meta8[0] is not None) == (f is not None)
             dy = torch.randn(y.shape, generator=torch.Generator().manual_seed(5)).to(y.dtype).to(dev)
             got.append((y.detach(),) + torch.autograd.grad(y, leaves, dy))
         A.set_activation_checkpoint(None)
@@ -300,3 +300,30 @@ def test_wgan_gp_steps_with_checkpoints(dev):
     o = tr.train_step(gb, gb)
     assert all(np.isfinite(float(o[k])) for k in ("g_loss", "d_loss"))
     lib.delete_all_params(); slim.reset_scopes()
+
+
+@pytest.mark.parametrize("fmt", [None, "e4m3", "int8"])
+def test_memory_held_between_forward_and_backward(dev, fmt):
+    """A block of 4096 x 512 holds its activations (4 tensors of 8 MiB in fp32, one of which the caller holds anyway) or 3 checkpoints of 33/32 MiB x 2; the
+    backward pass lets go of them although the loss lives on."""
+    A, H = _mods()
+    rows, C = 4096, 512
+    x = torch.randn(rows, C, device=dev).requires_grad_(True)
+    ws = [(0.05 * torch.randn(C, C, device=dev)).requires_grad_(True) for _ in range(2)]
+    ones = torch.ones(C, device=dev)
+
+    def run():
+        return A.gated_resblock(x, ones, None, ws[0], None, ws[1], None, ones, None, save8=fmt).sum()
+    run().backward()                                     # (workspaces, first gradients)
+    torch.cuda.synchronize()
+    empty = torch.cuda.memory_allocated()
+    loss = run()
+    held = torch.cuda.memory_allocated() - empty
+    tensor = rows * C * 4
+    stats = 4 * rows * 4 + 65536                         # mean and rstd twice; the loss and the allocator's roundings
+    if fmt is None:
+        assert 3 * tensor <= held <= 3 * tensor + stats
+    else:
+        assert held <= 3 * (tensor // 4 + tensor // 128) + stats
+    loss.backward()
+    assert torch.cuda.memory_allocated() - empty <= stats and float(loss) == float(loss)
