@@ -6,7 +6,6 @@
 #   stats      rocprofv3 --kernel-trace --stats of the headline (one stream), Market bf16, DeepFashion bf16, stage-II bf16
 #   pmc        matrix-pipe counters of the DeepFashion bf16 step AT HEAD with rocm-smi clock / power samples taken during the pass
 #   layers     per-layer tables (Market bf16, DeepFashion bf16, Market fp32)
-#   crash      scripts/diag_syncbn_graph_2rank.py (two ranks, SyncBN, captured graphs)
 #   bench      the driver's command, every information line
 R=${GRAFT_REPO_ROOT:-/root/repo}
 cd $R
@@ -53,8 +52,6 @@ layers)
   DPIG_WORKLOAD=market128 DPIG_DTYPE=f32w DPIG_TWO_STREAM=0 DPIG_D_OVERLAP=0 timeout 300 python scripts/layer_table.py > gpurun_out/profiles_out/r05_layer_market_f32w.txt 2>&1
   DPIG_WORKLOAD=market128 DPIG_DTYPE=f32 DPIG_TWO_STREAM=0 DPIG_D_OVERLAP=0 timeout 300 python scripts/layer_table.py > gpurun_out/profiles_out/r05_layer_market_f32.txt 2>&1
   head -3 gpurun_out/profiles_out/r05_layer_*.txt ;;
-crash)
-  timeout 600 python scripts/diag_syncbn_graph_2rank.py ${CRASH_ATTEMPTS:-8} graphs > gpurun_out/crash_graphs.log 2>&1; tail -60 gpurun_out/crash_graphs.log ;;
 bench)
   python bench.py --gpus 1 --steps 20 --warmup 5 > gpurun_out/profiles_out/r05_bench.json 2> gpurun_out/profiles_out/r05_bench.err
   tail -c 300 gpurun_out/profiles_out/r05_bench.err; python - <<'PY'

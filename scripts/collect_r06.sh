@@ -6,11 +6,8 @@
 #   stats      rocprofv3 --kernel-trace --stats of the headline (one stream), Market bf16, DeepFashion bf16, stage-II bf16
 #   pmc        matrix-pipe counters of the DeepFashion bf16 step AT HEAD with rocm-smi clock / power samples taken during the pass
 #   layers     per-layer tables (Market bf16, DeepFashion bf16, Market fp32)
-#   crash      scripts/diag_syncbn_graph_2rank.py (two ranks, SyncBN, captured graphs)
 #   bench      the driver's command, every information line
-#   guard      the guard-page sweeps: tests/guard/run_cases.py hi + lo (NaN-filled), the GPU suite per file on guard pages (both placements),
-#              the two-rank eager SyncBN step with every rank's allocations guarded
-#   crash50    scripts/diag_syncbn_graph_2rank.py 50 graphs -- VERDICT r5 #2's "50/50" bar for the two-rank captured step
+#   guard      the guard-page sweeps: tests/guard/run_cases.py hi + lo (NaN-filled), the GPU suite per file on guard pages (both placements)
 #   dry        scripts/run_scale.sh --dry (every branch of the 8-GPU script at N = 2 over gloo on this one GPU)
 # DPIG_HEAD=<git short hash> in the environment stamps the traffic entries (the GPU box has no .git)
 R=${GRAFT_REPO_ROOT:-/root/repo}
@@ -63,18 +60,10 @@ guard)
   for m in hi lo; do
     (time AMD_SERIALIZE_KERNEL=3 DPIG_GUARD_FILL=255 timeout 900 python tests/guard/run_cases.py $m) > gpurun_out/guard/cases_$m.log 2>&1
     echo "guard cases $m: OK $(grep -c '^OK' gpurun_out/guard/cases_$m.log) ERR $(grep -c '^ERR' gpurun_out/guard/cases_$m.log) $(grep '^DONE' gpurun_out/guard/cases_$m.log)"
-    DPIG_GUARD=$m AMD_SERIALIZE_KERNEL=3 DPIG_GUARD_FILL=255 timeout 600 python scripts/diag_syncbn_graph_2rank.py 6 eager > gpurun_out/guard/two_rank_eager_$m.log 2>&1
-    grep SUMMARY gpurun_out/guard/two_rank_eager_$m.log
     GUARD_FILE_TIMEOUT=600 bash scripts/guard_suite.sh $m > gpurun_out/guard/suite_$m.txt 2>&1; grep '^==' gpurun_out/guard/suite_$m.txt
   done ;;
-crash50)
-  timeout 1500 python scripts/diag_syncbn_graph_2rank.py 50 graphs > gpurun_out/crash50_graphs.log 2>&1
-  grep -E "^attempt|SUMMARY" gpurun_out/crash50_graphs.log | grep -v "\[0, 0\]" | tail -12
-  grep -B2 -A40 "log tail" gpurun_out/crash50_graphs.log | head -120 ;;
 dry)
   bash scripts/run_scale.sh --dry 2>&1 | tee gpurun_out/scale_dry.txt | tail -60 ;;
-crash)
-  timeout 600 python scripts/diag_syncbn_graph_2rank.py ${CRASH_ATTEMPTS:-8} graphs > gpurun_out/crash_graphs.log 2>&1; tail -60 gpurun_out/crash_graphs.log ;;
 bench)
   python bench.py --gpus 1 --steps 20 --warmup 5 > gpurun_out/profiles_out/r06_bench.json 2> gpurun_out/profiles_out/r06_bench.err
   cp gpurun_out/bench_info.jsonl gpurun_out/profiles_out/r06_bench_info.jsonl
