@@ -620,7 +620,8 @@ int dpig_transpose12(const void* x, void* y, int B, int A, int C, int elem_bytes
  * Beyond the reference's graph (its residual blocks, models.py:398-400 / 474-515, have neither norm nor gate): the same blocks with a norm over
  * the channels before and after, a gate and a residual scale, and activations kept for the backward pass in 8 bits.
  * Rows are every leading axis ([rows][C], a row stride ld* in elements, any alignment the element type allows); fp32 or bf16 tensors (is_bf16), fp32
- * parameters [C]; statistics and sums in fp32.  C is 1 .. 8192 where a norm is taken. */
+ * parameters [C]; statistics and sums in fp32.  C is 1 .. 8192 where a norm is taken.  A row tensor may be written in place of an operand at the same
+ * stride (y = x, out = x or f, dx = dy or accum, df = dout); other overlaps are not allowed. */
 #define DPIG_NORM_LAYER 0       /* xh = (x - mean) rstd                                                                  */
 #define DPIG_NORM_RMS 1         /* xh = x rstd, rstd = 1 / sqrt(mean_c x^2 + eps); mean pointers may be NULL               */
 

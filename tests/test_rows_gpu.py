@@ -414,3 +414,53 @@ def test_strided_results_leave_what_lies_between_their_rows(dev, bf16, C, ld):
     check(y, H.act8_load(a, dt))
     assert h.dpig_act8_act_bwd(P(dy), bf16, C, P(a.codes), rows, C, 1, 2, 0.2, P(inside(y)), ld, st) == 0
     check(y, H.act8_act_bwd(dy, a, 2))
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("rows,C,groups", [(3000, 37, 3000), (3000, 250, 6), (600, 1100, 20), (64, 512, 64)])
+def test_results_in_place_of_an_operand(dev, bf16, rows, C, groups):
+    """The C entries with y = x, out = x, out = f, df = dout, dx = dy and dx = accum give the bits of separate results."""
+    from dpig_amd import _lib
+    h, dt, H = _lib.lib(), BF16 if bf16 else F32, _H()
+    st = _lib.stream_ptr()
+    P = lambda t: t.data_ptr()      # noqa: E731
+    x, f, dy, acc = (_rand(rows, C, i, dt).to(dev) for i in (1, 2, 3, 4))
+    s, o, r = (_vec(C, i).to(dev) for i in (1, 2, 3))
+    gate = _rand(groups, C, 5).to(dev)
+    m, q = torch.empty(2, rows, device=dev).unbind(0)
+    y = H.rownorm_fwd(x, s, o)[0]
+    t = x.clone()
+    assert h.dpig_rownorm_fwd(P(t), bf16, C, rows, C, 0, P(s), P(o), EPS, P(t), C, P(m), P(q), 0, None, None, st) == 0
+    assert torch.equal(t, y)
+    out, mean, rstd, _, _ = H.gated_residual_fwd(x, f, s, o, gate, r)
+    for k in range(2):
+        a = [x.clone(), f.clone()]
+        assert h.dpig_gated_residual_fwd(P(a[0]), C, P(a[1]), C, bf16, rows, C, 0, P(s), P(o), EPS, P(gate), 0, groups, P(r), P(a[k]), C, P(m), P(q), 0, None,
+                                         None, 0, None, None, 0.0, None, 0, None, None, 0, None, None, st) == 0
+        assert torch.equal(a[k], out)
+    df = H.gated_residual_bwd(dy, f, s, o, gate, r, mean, rstd, want_params=False)[0]
+    t = dy.clone()
+    assert h.dpig_gated_residual_bwd(P(t), bf16, C, P(f), C, 0, None, None, rows, C, 0, P(s), P(o), P(gate), 0, groups, P(r), P(mean), P(rstd), P(t), C,
+                                     None, None, None, None, None, 0, st) == 0
+    assert torch.equal(t, df)
+    dx = H.rownorm_bwd(dy, f, s, mean, rstd, accum=acc, want_params=False)[0]
+    for k in range(2):
+        a = [dy.clone(), acc.clone()]
+        assert h.dpig_rownorm_bwd(P(a[0]), bf16, C, P(f), C, 0, None, None, rows, C, 0, P(s), P(mean), P(rstd), P(a[1]), C, P(a[k]), C, None, None, None, 0,
+                                  st) == 0
+        assert torch.equal(a[k], dx)
+
+
+def test_layers_without_rows(dev):
+    """No rows: empty results, zero gradients, through the autograd functions and the registry layers."""
+    from dpig_amd import autograd as A
+    for fmt in (None, "int8"):
+        x = torch.zeros(0, 64, device=dev, requires_grad=True)
+        f = torch.zeros(0, 64, device=dev, requires_grad=True)
+        s, o, r = (_vec(64, i).to(dev).requires_grad_(True) for i in (1, 2, 3))
+        h = A.rownorm(x, s, o, save8=fmt)
+        y = A.gated_residual(h, f, s, o, None, r, save8=fmt)
+        assert y.shape == (0, 64)
+        y.sum().backward()
+        assert x.grad.shape == (0, 64) and f.grad.shape == (0, 64)
+        assert all(float(t.grad.abs().sum()) == 0.0 for t in (s, o, r))
