@@ -11,7 +11,7 @@
 // The partials are added in a fixed order by one or two small launches: no atomics, the same bits every time.
 // Bound by HBM (2 to 4 row tensors in and out).  Measured, row pass + sums: 32768 x 384 fp32 with accum 39.0 + 4.2 us (201 MB, 5.2 TB/s in the pass);
 // 131072 x 256 bf16 with accum 52.0 + 4.3; 47915 x 250 bf16 from an int8 checkpoint 16.7 + 4.4; exit 32768 x 640 bf16 from its e4m3 checkpoint, a
-// gate per 4096 rows, 25.1 + 7.1 (105 MB, 4.2 TB/s); 32768 x 512 bf16 with a gate per row 44.7 + 4.8; 8192 x 2048 bf16 29.9 + 5.2.
+// gate per 4096 rows, 25.2 + 5.6 (105 MB, 4.2 TB/s); 32768 x 512 bf16 with a gate per row 44.7 + 4.8; 8192 x 2048 bf16 29.9 + 5.2.
 #pragma once
 #include "dpig_rows.h"
 

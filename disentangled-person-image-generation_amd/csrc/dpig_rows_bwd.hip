@@ -46,11 +46,37 @@ __device__ __forceinline__ void fin_add(const float (*red)[2][FC], int cl, float
 #pragma unroll
     for (int w = 0; w < FW; ++w) { *a += red[w][0][cl]; *b += red[w][1][cl]; }
 }
-__device__ __forceinline__ void fin_outputs(const FinP& p, int c, float a, float b) {
-    const float rs = p.res ? p.res[c] : 1.f;
-    if (p.dscale) p.dscale[c] = rs * a;
-    if (p.doffset) p.doffset[c] = rs * b;
-    if (p.dres) p.dres[c] = (p.scale ? p.scale[c] : 1.f) * a + (p.offset ? p.offset[c] : 0.f) * b;
+// a channel's parameters, asked for before the sums they are needed after
+struct FinChan {
+    float sc, of, rs;
+    __device__ __forceinline__ FinChan(const FinP& p, int c, bool in)
+        : sc(in && p.scale ? p.scale[c] : 1.f), of(in && p.offset ? p.offset[c] : 0.f), rs(in && p.res ? p.res[c] : 1.f) {}
+    __device__ __forceinline__ void outputs(const FinP& p, int c, float a, float b) const {
+        if (p.dscale) p.dscale[c] = rs * a;
+        if (p.doffset) p.doffset[c] = rs * b;
+        if (p.dres) p.dres[c] = sc * a + of * b;
+    }
+};
+// Sums of n pairs (A, B) `step` apart, in order, N of them on their way at a time: all loads of a batch are issued before the first is waited for (behind
+// the n-th the last one is read again and left out).  Left to itself the compiler waits for each pair: 7.1 us instead of 5.5 for 8 groups of 64.
+template <int N> __device__ __forceinline__ void fin_batch(const float* p, int C, long step, int n, float* a, float* b) {
+    float va[N], vb[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const float* q = p + min(u, n - 1) * step;
+        va[u] = q[0];
+        vb[u] = q[C];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        *a = u < n ? *a + va[u] : *a;
+        *b = u < n ? *b + vb[u] : *b;
+    }
+}
+__device__ __forceinline__ void fin_sums(const float* p, int C, long step, int n, float* a, float* b) {
+    for (; n > 2; n -= 8, p += 8 * step) fin_batch<8>(p, C, step, n, a, b);
+    if (n > 0) fin_batch<2>(p, C, step, n, a, b);
 }
 // pieces form with a gate: per group the sums over its pieces, dgate, and the gate-weighted sums over the groups of this workgroup.  `wpg` waves take a
 // group, four lanes a channel each, and sixteen / wpg groups are summed together with all their loads in flight; where every group is one
@@ -59,7 +85,7 @@ __global__ __launch_bounds__(FC * FL) void rows_groups_kernel(const FinP p) {
     __shared__ float red[1][FW][2][FC];
     const int cl = threadIdx.x % FC, ln = threadIdx.x / FC, c = blockIdx.x * FC + cl;
     const bool in = c < p.C;
-    const float sc = in && p.scale ? p.scale[c] : 1.f, of = in && p.offset ? p.offset[c] : 0.f, rs = in && p.res ? p.res[c] : 1.f;
+    const FinChan ch(p, c, in);
     const long g0 = blockIdx.y * p.gpb, g1 = min(g0 + p.gpb, p.ngroups);
     float wa = 0.f, wb = 0.f;
     auto gate_of = [&](long g) -> float {
@@ -69,7 +95,7 @@ __global__ __launch_bounds__(FC * FL) void rows_groups_kernel(const FinP p) {
     };
     auto close = [&](long g, float m, float a, float b) {
         if (p.dgate) {
-            const float t = rs * (sc * a + of * b);
+            const float t = ch.rs * (ch.sc * a + ch.of * b);
             if (p.gate_bf16) static_cast<bf16_t*>(p.dgate)[g * p.C + c] = f2bf(t);
             else static_cast<float*>(p.dgate)[g * p.C + c] = t;
         }
@@ -87,9 +113,8 @@ __global__ __launch_bounds__(FC * FL) void rows_groups_kernel(const FinP p) {
             const long g = gb + wave / p.wpg;
             float a[1] = {0.f}, b[1] = {0.f};
             if (in && g < g1) {
-                const float* src = p.partial + g * p.n * 2 * p.C + c;
-#pragma unroll 8
-                for (int s = part; s < (int)p.n; s += 4 * p.wpg) { a[0] += src[(long)s * 2 * p.C]; b[0] += src[((long)s * 2 + 1) * p.C]; }
+                const int each = 4 * p.wpg;
+                fin_sums(p.partial + (g * p.n + part) * 2 * p.C + c, p.C, 2L * each * p.C, ((int)p.n - part + each - 1) / each, &a[0], &b[0]);
             }
             fin_waves<1>(a, b, red);
             if (closer) {
@@ -103,21 +128,20 @@ __global__ __launch_bounds__(FC * FL) void rows_groups_kernel(const FinP p) {
     fin_waves<1>(a, b, red);
     if (!in || ln != 0) return;
     fin_add(red[0], cl, &wa, &wb);
-    if (gridDim.y == 1) { fin_outputs(p, c, wa, wb); return; }
+    if (gridDim.y == 1) { ch.outputs(p, c, wa, wb); return; }
     p.partial2[(long)blockIdx.y * 2 * p.C + c] = wa;
     p.partial2[((long)blockIdx.y * 2 + 1) * p.C + c] = wb;
 }
 __global__ __launch_bounds__(FC * FL) void rows_final_kernel(const FinP p) {
     __shared__ float red[1][FW][2][FC];
     const int cl = threadIdx.x % FC, ln = threadIdx.x / FC, c = blockIdx.x * FC + cl;
+    const FinChan ch(p, c, c < p.C);
     float a[1] = {0.f}, b[1] = {0.f};
-    if (c < p.C)
-#pragma unroll 4
-        for (long s = ln; s < p.n; s += FL) { a[0] += p.partial[s * 2 * p.C + c]; b[0] += p.partial[(s * 2 + 1) * p.C + c]; }
+    if (c < p.C) fin_sums(p.partial + 2L * ln * p.C + c, p.C, 2L * FL * p.C, (int)((p.n - ln + FL - 1) / FL), &a[0], &b[0]);
     fin_waves<1>(a, b, red);
     if (c >= p.C || ln != 0) return;
     fin_add(red[0], cl, a, b);
-    fin_outputs(p, c, a[0], b[0]);
+    ch.outputs(p, c, a[0], b[0]);
 }
 
 // ---- plan ------------------------------------------------------------------------------------------------------------------------------
@@ -154,7 +178,9 @@ static Plan plan(int64_t nrows, int C, bool gated, int64_t groups) {
     q.chunk = up(sets, pieces) * rpb;
     q.pieces = up(per, q.chunk);
     q.blocks = q.pieces * groups;
-    q.blocks2 = groups <= 2 * FW ? 1 : (groups / FW < 256 ? groups / FW : 256);
+    // (where a group is one piece, a lane takes a group: sixteen times as many of them keep a workgroup of the sums busy)
+    q.blocks2 = groups <= 2 * FW ? 1 : q.pieces == 1 ? up(groups, FL) : groups / FW;
+    if (q.blocks2 > 256) q.blocks2 = 256;
     return q;
 }
 static size_t ws_bytes(const Plan& q, int C) {
