@@ -22,6 +22,7 @@ Arithmetic modes (`set_compute`):
            mode, held to the exact path's kernel bar (2e-5 max|ref|); 'f32' stays the exact-products default.
 """
 import ctypes
+import functools
 import os
 
 import torch
@@ -1505,6 +1506,12 @@ def _new_act8(shape, rows, C, fmt, device):
     return a
 
 
+@functools.lru_cache(maxsize=1024)
+def _ws_bytes(query, *sizes):
+    """What a workspace query of the library answers: it depends on the sizes alone, and asking costs a microsecond a call."""
+    return getattr(lib(), query)(*sizes)
+
+
 def _scratch(nbytes, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
@@ -1526,7 +1533,7 @@ def act8_store(x, fmt="e4m3"):
     dev = x.device
     a = _new_act8(x.shape, rows, C, fmt, dev)
     if rows:
-        check(lib().dpig_act8_store(ptr(x), int(x.dtype == BF16), ld, rows, C, f, ptr(a.codes), ptr(a.scales), _lib.raw_stream(dev.index)), "act8_store")
+        check(lib().dpig_act8_store(x.data_ptr(), int(x.dtype == BF16), ld, rows, C, f, a.codes.data_ptr(), a.scales.data_ptr(), _lib.raw_stream(dev.index)), "act8_store")
     return a
 
 
@@ -1546,7 +1553,7 @@ def act8_load(a, dtype=F32):
     y = torch.empty(a.shape, dtype=dtype, device=dev)
     rows, C = a.codes.shape[0], a.shape[-1]
     if rows:
-        check(lib().dpig_act8_load(ptr(a.codes), ptr(a.scales), rows, C, _fmt8(a.fmt), ptr(y), int(dtype == BF16), C, _lib.raw_stream(dev.index)), "act8_load")
+        check(lib().dpig_act8_load(a.codes.data_ptr(), a.scales.data_ptr(), rows, C, _fmt8(a.fmt), y.data_ptr(), int(dtype == BF16), C, _lib.raw_stream(dev.index)), "act8_load")
     return y
 
 
@@ -1561,7 +1568,7 @@ def act8_act_bwd(dy, a, act, alpha=0.2):
     _act8_on(a, dev)
     dz = _like_rows(dy)
     if rows:
-        check(lib().dpig_act8_act_bwd(ptr(dy), int(dy.dtype == BF16), ld, ptr(a.codes), rows, C, _fmt8(a.fmt), act, alpha, ptr(dz), C,
+        check(lib().dpig_act8_act_bwd(dy.data_ptr(), int(dy.dtype == BF16), ld, a.codes.data_ptr(), rows, C, _fmt8(a.fmt), act, alpha, dz.data_ptr(), C,
                                       _lib.raw_stream(dev.index)), "act8_act_bwd")
     return dz
 
@@ -1591,9 +1598,9 @@ def linear_wgrad8(a, dy, scale=None, offset=None, out=None, beta=0.0, want_bias=
         return (out, db) if want_bias else out
     bf = int(dy.dtype == BF16)
     affine = int(scale is not None or offset is not None)
-    nbytes = lib().dpig_linear_wgrad8_workspace_bytes(rows, C, ld, K, bf, affine)
+    nbytes = _ws_bytes("dpig_linear_wgrad8_workspace_bytes", rows, C, ld, K, bf, affine)
     ws = _scratch(nbytes, dev)
-    check(lib().dpig_linear_wgrad8(ptr(a.codes), ptr(a.scales), _fmt8(a.fmt), rows, C, ptr(dy), bf, ld, K, ptr(scale), ptr(offset), ptr(out),
+    check(lib().dpig_linear_wgrad8(a.codes.data_ptr(), a.scales.data_ptr(), _fmt8(a.fmt), rows, C, dy.data_ptr(), bf, ld, K, ptr(scale), ptr(offset), out.data_ptr(),
                                    float(beta), ptr(db), float(db_beta), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "linear_wgrad8")
     return (out, db) if want_bias else out
 
@@ -1610,7 +1617,7 @@ def rownorm_fwd(x, scale=None, offset=None, eps=1e-5, kind="layer", save8=None):
     mean, rstd = _vectors(2, rows, dev) if k == 0 else (None, torch.empty(rows, dtype=F32, device=dev))
     a = _new_act8(x.shape, rows, C, save8, dev) if save8 is not None else None
     if rows:
-        check(lib().dpig_rownorm_fwd(ptr(x), int(x.dtype == BF16), ld, rows, C, k, ptr(scale), ptr(offset), eps, ptr(y), C, ptr(mean), ptr(rstd),
+        check(lib().dpig_rownorm_fwd(x.data_ptr(), int(x.dtype == BF16), ld, rows, C, k, ptr(scale), ptr(offset), eps, y.data_ptr(), C, ptr(mean), rstd.data_ptr(),
                                      f, ptr(a.codes) if a else None, ptr(a.scales) if a else None, _lib.raw_stream(dev.index)), "rownorm_fwd")
     return y, mean, rstd, a
 
@@ -1647,10 +1654,10 @@ def rownorm_bwd(dy, saved, scale, mean, rstd, kind="layer", accum=None, want_par
         if want_params:
             dscale.zero_(), doffset.zero_()
         return dx, dscale, doffset
-    nbytes = lib().dpig_rownorm_bwd_workspace_bytes(rows, C) if want_params else 0
+    nbytes = _ws_bytes("dpig_rownorm_bwd_workspace_bytes", rows, C) if want_params else 0
     ws = _scratch(nbytes, dev)
-    check(lib().dpig_rownorm_bwd(ptr(dy), int(dy.dtype == BF16), ld, xp, ldx, f, codes, scales, rows, C, k, ptr(scale), ptr(mean), ptr(rstd),
-                                 ptr(accum), lda, ptr(dx), C, ptr(dscale), ptr(doffset), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "rownorm_bwd")
+    check(lib().dpig_rownorm_bwd(dy.data_ptr(), int(dy.dtype == BF16), ld, xp, ldx, f, codes, scales, rows, C, k, ptr(scale), ptr(mean), rstd.data_ptr(),
+                                 ptr(accum), lda, dx.data_ptr(), C, ptr(dscale), ptr(doffset), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "rownorm_bwd")
     return dx, dscale, doffset
 
 
@@ -1701,8 +1708,8 @@ def gated_residual_fwd(x, f, scale=None, offset=None, gate=None, res_scale=None,
         raise RuntimeError("gated_residual_fwd: next_save8 without next_norm")
     if rows:
         check(lib().dpig_gated_residual_fwd(
-            ptr(x), ldx, ptr(f), ldf, int(x.dtype == BF16), rows, C, k, ptr(scale), ptr(offset), eps, ptr(gate),
-            int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(out), C, ptr(mean), ptr(rstd), q, ptr(a.codes) if a else None,
+            x.data_ptr(), ldx, f.data_ptr(), ldf, int(x.dtype == BF16), rows, C, k, ptr(scale), ptr(offset), eps, ptr(gate),
+            int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), out.data_ptr(), C, ptr(mean), rstd.data_ptr(), q, ptr(a.codes) if a else None,
             ptr(a.scales) if a else None, k2, ptr(scale2), ptr(offset2), eps2, ptr(h), C, ptr(mean2), ptr(rstd2), q2,
             ptr(a2.codes) if a2 else None, ptr(a2.scales) if a2 else None, _lib.raw_stream(dev.index)), "gated_residual_fwd")
     return out, mean, rstd, a, ((h, mean2, rstd2, a2) if next_norm is not None else None)
@@ -1733,11 +1740,11 @@ def gated_residual_bwd(dout, saved, scale, offset, gate, res_scale, mean, rstd, 
             if t is not None:
                 t.zero_()
         return df, dscale, doffset, dgate, dres
-    nbytes = lib().dpig_gated_residual_bwd_workspace_bytes(rows, C, groups) if want_params else 0
+    nbytes = _ws_bytes("dpig_gated_residual_bwd_workspace_bytes", rows, C, groups) if want_params else 0
     ws = _scratch(nbytes, dev)
     check(lib().dpig_gated_residual_bwd(
-        ptr(dout), int(dout.dtype == BF16), ld, fp, ldf, q, codes, scales, rows, C, k, ptr(scale), ptr(offset), ptr(gate),
-        int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(mean), ptr(rstd), ptr(df), C, ptr(dscale), ptr(doffset), ptr(dgate),
+        dout.data_ptr(), int(dout.dtype == BF16), ld, fp, ldf, q, codes, scales, rows, C, k, ptr(scale), ptr(offset), ptr(gate),
+        int(gate is not None and gate.dtype == BF16), groups, ptr(res_scale), ptr(mean), rstd.data_ptr(), df.data_ptr(), C, ptr(dscale), ptr(doffset), ptr(dgate),
         ptr(dres), ptr(ws), nbytes, _lib.raw_stream(dev.index)), "gated_residual_bwd")
     return df, dscale, doffset, dgate, dres
 
