@@ -12,13 +12,15 @@
 // way into LDS) and read with the transposing LDS read.  The rows are split over workgroups until the chip is full; partial sums are
 // joined by a second launch in a fixed order.
 //
-// Measured, product + join: bf16 dy 131072 x 512 x 512 82.5 + 6.6 us (68.7 GFLOP: 833 TFLOP/s in the product; a library product of two bf16
-// operands of that shape takes 361 us), 131072 x 768 x 768 172 us in all (900 TFLOP/s), 32768 x 512 x 512 34, 2048 x 512 x 512 14.7; fp32 dy
-// 131072 x 256 x 256 52.0 + 7.1, 32768 x 512 x 512 49.2 + 6.5 (349 TFLOP/s of fp32 products), 20011 x 250 x 390 23.0 + 5.7.
-// Of the large product's 82.5 us the matrix instructions and barriers alone take 54, without the loads it is 69, without decoding and
-// staging 63: the matrix pipe, the LDS port and the loads' waits overlap, but not fully.  Asking L2 for tiles ahead of the loads changed nothing.
+// Measured, product + join: bf16 dy 131072 x 512 x 512 79.4 + 6.6 us (68.7 GFLOP: 865 TFLOP/s in the product; a library product of two bf16
+// operands of that shape takes 361 us), 131072 x 768 x 768 169 us in all (915 TFLOP/s), 32768 x 512 x 512 34, 2048 x 512 x 512 14.7; fp32 dy
+// 131072 x 128 x 128 21.9 + 6.1, 32768 x 512 x 512 47.3 + 6.6 (363 TFLOP/s of fp32 products), 20011 x 250 x 390 22.4 + 5.7.
+// Of the large product the matrix instructions and barriers alone take 54 us, without the loads it is 69, without decoding and staging 63: the
+// matrix pipe, the LDS port and the loads' waits overlap, but not fully.  Asking L2 for tiles ahead of the loads, or for three and six tiles ahead
+// instead of two, changed nothing.  (The steps of the loop as one expression, one exit behind each: 79.4 us; with a branch of its own each, 82.3.)
 #include "dpig_rows.h"
 #include <type_traits>
+#include <utility>
 
 namespace dpig {
 namespace wg8 {
@@ -77,6 +79,11 @@ template <int I, int NM, int NW, int NL> __device__ __forceinline__ void weave()
         if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
         weave<I + 1, NM, NW, NL>();
     }
+}
+
+// step(0) && step(1) && ...
+template <typename S, int... I> __device__ __forceinline__ bool every(S& step, std::integer_sequence<int, I...>) {
+    return (step(std::integral_constant<int, I>()) && ...);
 }
 
 // Eight waves, WM x 8 / WM, each with MA x NB blocks of 32 x 32; TR rows per tile.
@@ -330,16 +337,7 @@ __global__ __launch_bounds__(512, 2) void wgrad8_kernel(const P p) {
         barrier();
         return ++t < ntr;
     };
-    for (;;) {
-        if (!step(std::integral_constant<int, 0>())) break;
-        if (!step(std::integral_constant<int, 1>())) break;
-        if constexpr (LATE) {
-            if (!step(std::integral_constant<int, 2>())) break;
-            if (!step(std::integral_constant<int, 3>())) break;
-            if (!step(std::integral_constant<int, 4>())) break;
-            if (!step(std::integral_constant<int, 5>())) break;
-        }
-    }
+    while (every(step, std::make_integer_sequence<int, LATE ? 6 : 2>())) {}
     if (wave < 4) barrier();
 
     // ---- result: accumulator register r of lane (half, l31) is row (r & 3) + 8 (r >> 2) + 4 half, column l31 of its 32x32 block ----------
