@@ -173,6 +173,9 @@ __device__ __forceinline__ void whiten(float (&v)[NV][8], const int (&n)[NV], fl
     *rstd = r;
 }
 
+// The checkpoint is of xh as rounded to fp32: one value in about 10^6 lies so near the edge between two codes that this, and the last bits of the
+// statistics, decide which it gets (141 of 127 million values against sums and products in 64 bits; 153 for elementary operations in fp32).
+// Products rounded to odd bring it to 102 and cost the 131072 x 256 bf16 norm 37.2 us instead of 30.7.
 // One vector of a row into its checkpoint; the four lanes of a quad hold the 32 channels of a group.  `in`: the vector lies within
 // the padded row (the same for the whole quad).
 template <int F> __device__ __forceinline__ void save8_as(const float (&v)[8], uint8_t* code, uint8_t* scale, bool first) {
