@@ -19,11 +19,23 @@
 // (never reused: use-after-free faults too).  Build: __graft_entry__.build_guard().
 #include <hip/hip_runtime.h>
 
+#include <cstdint>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <unordered_map>
+
+// The layout of one allocation in units of bytes from its reservation's base, arithmetic alone (tests/test_guard_host.py):
+// [0, mapped_at) unmapped | [mapped_at, mapped_at + mapped) mapped | [.., reserved) unmapped, the tensor at `tensor_at`.
+struct GuardPlace { uint64_t reserved, mapped_at, mapped, tensor_at; };
+extern "C" void dpig_guard_place(uint64_t size, uint64_t granularity, int at_start, GuardPlace* out) {
+    if (size == 0) size = 1;
+    out->mapped = (size + granularity - 1) / granularity * granularity;
+    out->reserved = out->mapped + 2 * granularity;
+    out->mapped_at = granularity;
+    out->tensor_at = at_start ? granularity : granularity + out->mapped - (size + 15) / 16 * 16;
+}
 
 namespace {
 
@@ -60,12 +72,15 @@ extern "C" void* dpig_guard_alloc(ssize_t size, int device, hipStream_t stream) 
     prop.location.id = device;
     if (!g_gran) GCHECK(hipMemGetAllocationGranularity(&g_gran, &prop, hipMemAllocationGranularityMinimum));
     const size_t g = g_gran;
+    const char* mode = std::getenv("DPIG_GUARD_MODE");
+    GuardPlace at;
+    dpig_guard_place((uint64_t)size, g, mode && std::strcmp(mode, "lo") == 0, &at);
     Rec r;
-    r.mapped = ((size_t)size + g - 1) / g * g;
-    r.reserved = r.mapped + 2 * g;
+    r.mapped = at.mapped;
+    r.reserved = at.reserved;
     GCHECK(hipMemAddressReserve(&r.base, r.reserved, g, nullptr, 0));
     GCHECK(hipMemCreate(&r.handle, r.mapped, &prop, 0));
-    char* lo = (char*)r.base + g;
+    char* lo = (char*)r.base + at.mapped_at;
     GCHECK(hipMemMap(lo, r.mapped, 0, r.handle, 0));
     hipMemAccessDesc acc;
     std::memset(&acc, 0, sizeof(acc));
@@ -76,10 +91,7 @@ extern "C" void* dpig_guard_alloc(ssize_t size, int device, hipStream_t stream) 
     if (fill && *fill) {
         GCHECK(hipMemsetAsync(lo, std::atoi(fill) & 255, r.mapped, stream));
     }
-    const char* mode = std::getenv("DPIG_GUARD_MODE");
-    const bool at_start = mode && std::strcmp(mode, "lo") == 0;
-    const size_t sz16 = ((size_t)size + 15) / 16 * 16;
-    void* p = at_start ? (void*)lo : (void*)(lo + r.mapped - sz16);
+    void* p = (char*)r.base + at.tensor_at;
     g_live[p] = r;
     ++g_count;
     g_bytes += (long)r.mapped;
