@@ -58,9 +58,11 @@ layers)
 guard)
   mkdir -p gpurun_out/guard
   for m in hi lo; do
-    (time AMD_SERIALIZE_KERNEL=3 DPIG_GUARD_FILL=255 timeout 900 python tests/guard/run_cases.py $m) > gpurun_out/guard/cases_$m.log 2>&1
+    (time AMD_SERIALIZE_KERNEL=3 DPIG_GUARD_FILL=255 timeout -k 10 900 python tests/guard/run_cases.py $m) > gpurun_out/guard/cases_$m.log 2>&1; rc=$?
     echo "guard cases $m: OK $(grep -c '^OK' gpurun_out/guard/cases_$m.log) ERR $(grep -c '^ERR' gpurun_out/guard/cases_$m.log) $(grep '^DONE' gpurun_out/guard/cases_$m.log)"
-    GUARD_FILE_TIMEOUT=600 bash scripts/guard_suite.sh $m > gpurun_out/guard/suite_$m.txt 2>&1; grep '^==' gpurun_out/guard/suite_$m.txt
+    [ $rc -eq 0 ] || exit $rc                                  # (nothing more on the GPU behind a fault)
+    GUARD_FILE_TIMEOUT=600 bash scripts/guard_suite.sh $m > gpurun_out/guard/suite_$m.txt 2>&1; rc=$?; grep '^==' gpurun_out/guard/suite_$m.txt
+    [ $rc -eq 0 ] || exit $rc
   done ;;
 dry)
   bash scripts/run_scale.sh --dry 2>&1 | tee gpurun_out/scale_dry.txt | tail -60 ;;

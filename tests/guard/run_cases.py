@@ -5,8 +5,8 @@ parameter / gradient / Adam buffer, channel slice -- is a deterministic `Memory 
     AMD_SERIALIZE_KERNEL=3 python tests/guard/run_cases.py hi|lo [first_case [last_case]]
 
 Prints `CASE <i> <name>` before and `OK <i> <name>` after each case (device synchronised), `DONE <n>` at the end; faulthandler is on, so
-a fault also prints the Python stack of the launching call.  tests/test_guard_gpu.py runs this in a sub-process for both placements and
-restarts after a faulting case so that ONE run lists every faulting case.
+a fault also prints the Python stack of the launching call.  tests/test_guard_gpu.py runs this in a sub-process for both placements; a
+faulting case ends the sweep.
 """
 import faulthandler
 import os

@@ -1,8 +1,10 @@
-"""The guard-page harness (tests/guard) without a GPU: where the allocator puts a tensor between its unmapped pages, and that no GPU test reads
-outside of one."""
+"""The guard-page harness (tests/guard) without a GPU: where the allocator puts a tensor between its unmapped pages, that no GPU test reads
+outside of one, and that nothing runs behind a fault."""
 import ctypes
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 
@@ -45,3 +47,29 @@ def test_no_gpu_test_copies_from_behind_a_guarded_tensor():
     text = open(os.path.join(ROOT, "tests", "test_guard_gpu.py")).read()
     offsets = re.findall(r'"-c", code, str\(([^)]*)\)', text)
     assert offsets and all(0 <= eval(o) <= 4096 - 16 for o in offsets), offsets
+
+
+def test_a_sweep_ends_with_its_first_faulting_case(monkeypatch):
+    sys.path.insert(0, os.path.join(ROOT, "tests"))
+    import test_guard_gpu as G
+    runs = []
+
+    def dies(cmd, **kw):
+        runs.append(cmd)
+        assert len(runs) == 1, "started again behind a fault"
+        return subprocess.CompletedProcess(cmd, -6, stdout="CASE 0 a\nOK 0 a\nCASE 1 b\nERR 1 b: x\nCASE 2 c\n", stderr="Memory access fault\n")
+    monkeypatch.setattr(G.subprocess, "run", dies)
+    faults, errs, total = G.sweep("hi")
+    assert len(faults) == 1 and faults[0].startswith("2 c [rc -6] Memory access fault") and errs == ["ERR 1 b: x"] and total is None
+
+
+@pytest.mark.parametrize("status,ran", [(0, 3), (5, 3), (1, 2), (134, 2), (124, 2)])
+def test_the_suite_on_guard_pages_stops_at_the_first_failing_file(tmp_path, status, ran):
+    """The second of three files ends with `status` (5: nothing selected); a stand-in for python counts the calls."""
+    fake = tmp_path / "python"
+    fake.write_text("#!/bin/sh\necho run >> %s/calls\n[ $(wc -l < %s/calls) -eq 2 ] && exit %d\nexit 0\n" % (tmp_path, tmp_path, status))
+    fake.chmod(0o755)
+    env = dict(os.environ, PATH="%s:%s" % (tmp_path, os.environ["PATH"]), GRAFT_REPO_ROOT=str(tmp_path))
+    r = subprocess.run(["bash", os.path.join(ROOT, "scripts", "guard_suite.sh"), "hi", "a.py", "b.py", "c.py"], env=env, capture_output=True, text=True)
+    assert len((tmp_path / "calls").read_text().split()) == ran, r.stdout + r.stderr
+    assert r.returncode == (0 if status in (0, 5) else status)
