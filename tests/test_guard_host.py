@@ -73,3 +73,10 @@ def test_the_suite_on_guard_pages_stops_at_the_first_failing_file(tmp_path, stat
     r = subprocess.run(["bash", os.path.join(ROOT, "scripts", "guard_suite.sh"), "hi", "a.py", "b.py", "c.py"], env=env, capture_output=True, text=True)
     assert len((tmp_path / "calls").read_text().split()) == ran, r.stdout + r.stderr
     assert r.returncode == (0 if status in (0, 5) else status)
+
+
+def test_no_script_is_there_to_bring_a_fault_out():
+    """Programs that load the GPU without torch's caching allocator, so that a stray access leaves mapped memory, are the guard-page tests alone."""
+    held = [f for f in os.listdir(os.path.join(ROOT, "scripts")) if f.endswith((".py", ".sh"))
+            and "NO_CUDA_MEMORY_CACHING" in open(os.path.join(ROOT, "scripts", f)).read()]
+    assert not held
