@@ -572,8 +572,9 @@ class DPIG_Encoder_GAN_BodyROI_FgBg(object):
         return bool(A._SYNC_BN_GROUP[0]) and self.allreduce.enabled
 
     def _capture(self, fn, pool=None):
-        """(replayable, fn's result): one hipGraph -- or, with cross-rank batch-norm statistics, a chain of graphs with the statistics'
-        all-reduces between them (autograd.SegmentedCapture: the critic's BatchNorm layers are `eager_island`s)."""
+        """(replayable, fn's result): one hipGraph -- or, with cross-rank batch-norm statistics (in a world of one rank, see
+        `enable_graphs`), a chain of graphs with the statistics' all-reduces between them (autograd.SegmentedCapture: the critic's
+        BatchNorm layers are `eager_island`s)."""
         if getattr(self, "_cap_stream", None) is None:
             # ONE capture stream for every graph of this trainer: a later graph's backward pass replays nodes on the stream they
             # were recorded on (an earlier capture's), which must be the stream being captured
@@ -593,7 +594,12 @@ class DPIG_Encoder_GAN_BodyROI_FgBg(object):
         cost of ~900 launches.  Single GPU: one graph per optimizer op (fwd + bwd + Adam).  Data parallel:
         the graph stops after the backward pass; the RCCL all-reduce of the flat gradient buffer and the
         Adam launch follow eagerly on the same stream (collectives are kept out of the capture).
-        Inputs are copied into static buffers; outputs are static tensors overwritten by each replay."""
+        Inputs are copied into static buffers; outputs are static tensors overwritten by each replay.
+        Cross-rank batch-norm statistics over several ranks are refused: a rank of such a captured step has died with a GPU memory access
+        fault whose cause is not known (the eager step has not)."""
+        if self._sync_bn_active() and self.allreduce.world > 1:
+            raise RuntimeError("enable_graphs: captured steps with batch-norm statistics over %d ranks are not supported; run them eagerly or "
+                               "with sync_bn=False" % self.allreduce.world)
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream(self.device))
         self._static_g = {k: v.clone() for k, v in batch_g.items()}
