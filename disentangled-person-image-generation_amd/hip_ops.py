@@ -1573,9 +1573,28 @@ def act8_act_bwd(dy, a, act, alpha=0.2):
     return dz
 
 
+WGRAD8_MOST, WGRAD8_STRIDE = 32768, 1 << 22          # channels and columns, and row stride of dy, that the kernel takes
+
+
+def _wgrad8_decoded(a, dy, scale, offset, out, beta, db, db_beta):
+    """linear_wgrad8 of matrices wider than its kernel takes (the fully connected layer behind a 16 x 16 x 640 map has 163840 inputs, and few rows): the
+    values are decoded, and linear_wgrad and colsum do the rest."""
+    rows, C = a.codes.shape[0], a.shape[-1]
+    x = act8_load(a).view(rows, C)
+    if scale is not None:
+        x.mul_(scale.view(C))
+    if offset is not None:
+        x.add_(offset.view(C))
+    dy = dy.reshape(rows, -1)
+    linear_wgrad(x, dy, out=out, beta=beta)
+    if db is not None:
+        colsum(dy, out=db, beta=db_beta)
+
+
 def linear_wgrad8(a, dy, scale=None, offset=None, out=None, beta=0.0, want_bias=False, db=None, db_beta=0.0):
     """dw[C, K] = beta * dw + x^T @ dy with x = scale * (the checkpoint's values) + offset, in fp32; `want_bias`: (dw, db) with the column sums
-    db[K] = db_beta * db + sum dy.  dy fp32 or bf16, rows as the checkpoint's.  `out` / `db`: contiguous fp32 buffers to write or add into."""
+    db[K] = db_beta * db + sum dy.  dy fp32 or bf16, rows as the checkpoint's.  `out` / `db`: contiguous fp32 buffers to write or add into.
+    Above 32768 channels or columns the values are decoded first (fp32, rows x C) and multiplied as linear_wgrad does."""
     dy, rows, K, ld = _rows_of(dy, "dy")
     C = a.shape[-1]
     if rows != a.codes.shape[0]:
@@ -1596,6 +1615,11 @@ def linear_wgrad8(a, dy, scale=None, offset=None, out=None, beta=0.0, want_bias=
             if t is not None:
                 t.mul_(b) if b else t.zero_()
         return (out, db) if want_bias else out
+    if C > WGRAD8_MOST or K > WGRAD8_MOST:
+        _wgrad8_decoded(a, dy, scale, offset, out, beta, db, db_beta)
+        return (out, db) if want_bias else out
+    if ld > WGRAD8_STRIDE:
+        dy, ld = dy.contiguous(), K
     bf = int(dy.dtype == BF16)
     affine = int(scale is not None or offset is not None)
     nbytes = _ws_bytes("dpig_linear_wgrad8_workspace_bytes", rows, C, ld, K, bf, affine)

@@ -671,7 +671,7 @@ int dpig_gated_residual_bwd(const void* dout, int is_bf16, int64_t lddo, const v
 /* Filter gradient from a checkpoint: dw[C][K] = beta * dw + sum_r (scale * q + offset)[r][c] * dy[r][k] (scale / offset [C], NULL: 1 / 0), and
  * db[K] = beta_b * db + sum_r dy (NULL: not wanted).  The result is that of fp32 products and sums for fp32 and bf16 dy alike
  * (an infinite fp32 dy gives NaN).
- * `affine` of the query: scale or offset is given. */
+ * C and K up to 32768, lddy up to 2^22, rows up to 2^30.  `affine` of the query: scale or offset is given. */
 size_t dpig_linear_wgrad8_workspace_bytes(int64_t rows, int C, int64_t lddy, int K, int dy_bf16, int affine);
 int dpig_linear_wgrad8(const uint8_t* codes, const uint8_t* scales, int fmt, int64_t rows, int C, const void* dy, int dy_bf16, int64_t lddy,
                        int K, const float* scale, const float* offset, float* dw, float beta, float* db, float beta_b, void* ws,

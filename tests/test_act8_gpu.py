@@ -249,3 +249,37 @@ def test_refusals(dev):
                  lambda: H.Act8(a.codes[:, :32], a.scales, (6, 40), "e4m3"), lambda: H.Act8(a.codes, a.scales, (5, 40), "e4m3")):
         with pytest.raises(RuntimeError):
             call()
+
+
+# the 256 x 256 generator's fully connected layer has 163840 inputs at its full width: more than a checkpoint's product takes (32768)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C,K", [(5, 40000, 3), (33, 40, 40000), (64, 32769, 33), (1, 163840, 64)])
+def test_linear_wgrad8_of_wide_matrices_is_exact_on_integers(dev, rows, C, K, dtype):
+    H = _H()
+    g = torch.Generator(device=dev).manual_seed(rows)
+    q = torch.randint(-8, 9, (rows, C), generator=g, device=dev).float()
+    dy = torch.randint(-3, 4, (rows, K), generator=g, device=dev)
+    scale, offset = (torch.randint(1, 4, (C,), generator=g, device=dev).float() for _ in range(2))
+    a, d = H.act8_store(q, "int8"), dy.to(dtype)
+    want, sums = q.double().t().contiguous() @ dy.double(), dy.double().sum(0)
+    assert torch.equal(H.linear_wgrad8(a, d).double(), want)
+    dw, db = H.linear_wgrad8(a, d, scale=scale, offset=offset, want_bias=True)
+    affine = want * scale.double()[:, None] + offset.double()[:, None] * sums
+    assert torch.equal(dw.double(), affine) and torch.equal(db.double(), sums)
+    out, b = torch.full((C, K), 2.0, device=dev), torch.full((K,), 3.0, device=dev)
+    r = H.linear_wgrad8(a, d, offset=offset, out=out, beta=0.5, db=b, db_beta=2.0)
+    assert r[0] is out and r[1] is b
+    assert torch.equal(out.double(), want + offset.double()[:, None] * sums + 1) and torch.equal(b.double(), sums + 6)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_wgrad8_of_rows_far_apart(dev, dtype):
+    """Rows of dy more than 2^22 elements apart: copied together first."""
+    H = _H()
+    g = torch.Generator(device=dev).manual_seed(1)
+    ld, rows = (1 << 22) + 64, 4
+    q, dy = torch.randint(-8, 9, (rows, 40), generator=g, device=dev).float(), torch.randint(-3, 4, (rows, 24), generator=g, device=dev).to(dtype)
+    wide = torch.empty(rows * ld, dtype=dtype, device=dev).as_strided((rows, 24), (ld, 1))
+    wide.copy_(dy)
+    dw, db = H.linear_wgrad8(H.act8_store(q, "int8"), wide, want_bias=True)
+    assert torch.equal(dw.double(), q.double().t().contiguous() @ dy.double()) and torch.equal(db.double(), dy.double().sum(0))

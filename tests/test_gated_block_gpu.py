@@ -327,3 +327,36 @@ def test_memory_held_between_forward_and_backward(dev, fmt):
         assert held <= 3 * (tensor // 4 + tensor // 128) + stats
     loss.backward()
     assert torch.cuda.memory_allocated() - empty <= stats and float(loss) == float(loss)
+
+
+def test_layers_wider_than_a_checkpoints_product(dev):
+    """linear(save8=) with 40960 features in and out, and the 256 x 256 model, whose generator flattens its 16 x 16 map into as many (here at a
+    quarter of its width): a training step with checkpoints runs and keeps the generator's first loss."""
+    A, H = _mods()
+    g = torch.Generator(device=dev).manual_seed(1)
+    for C, F in ((40960, 24), (24, 40960)):
+        x = torch.randint(-8, 9, (6, C), generator=g, device=dev).float().requires_grad_(True)
+        w = torch.randint(-2, 3, (C, F), generator=g, device=dev).float().requires_grad_(True)
+        b = torch.zeros(F, device=dev, requires_grad=True)
+        dy = torch.randint(-3, 4, (6, F), generator=g, device=dev).float()
+        A.linear(x, w, b, save8="int8").backward(dy)
+        assert torch.equal(w.grad.double(), x.detach().double().t().contiguous() @ dy.double())
+        assert torch.equal(b.grad.double(), dy.double().sum(0)) and torch.equal(x.grad.double(), dy.double() @ w.detach().double().t().contiguous())
+    import dpig_amd.tflib as lib
+    from dpig_amd import slim, synthetic
+    from dpig_amd.trainer import Config
+    from dpig_amd.trainer_256 import DPIG_Encoder_GAN_BodyROI_256
+    first = []
+    for fmt in (None, "e4m3"):
+        lib.delete_all_params(); slim.reset_scopes(); lib.set_device(dev)
+        np.random.seed(1)
+        tr = DPIG_Encoder_GAN_BodyROI_256(Config(batch_size=1, img_H=256, img_W=256, conv_hidden_num=32, z_num=8, act_checkpoint=fmt), dev)
+        gb = synthetic.to_device(synthetic.make_batch(1, img_H=256, img_W=256, seed=3), dev)
+        tr.init_net(gb)
+        tr.step = 1
+        assert max(p.shape[0] for n, p in lib._params.items() if n.endswith("fully_connected/weights")) == 40960
+        o = tr.train_step(gb, gb)
+        first.append(float(o["g_loss"]))
+        assert np.isfinite(float(o["d_loss"])) and bool(torch.isfinite(tr.G_flat.flat).all())
+    assert first[0] == first[1]
+    lib.delete_all_params(); slim.reset_scopes()
