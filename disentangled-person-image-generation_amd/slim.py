@@ -148,16 +148,18 @@ def gated_res_block(inputs, num_hidden=None, gate=None, activation_fn=relu, kind
     residual scale (beyond the reference):
         x + res_scale * gate * (norm(fc(act(fc(norm(x) * s1 + o1)))) * s2 + o2)
     inputs [..., C] (rows of channels), `num_hidden` the inner width (default C), gate [C], [G, C] or as inputs (None: 1), e.g. a fully_connected
-    of a conditioning vector.  Variables `<scope>/GatedResidual[_k]/{entry_scale, entry_offset, exit_scale, exit_offset, res_scale}` and two
-    `fully_connected[_k]/{weights, biases}`; res_scale starts at 0.1.  `save8` ('e4m3' | 'int8'): activations kept in 8 bits for the
-    backward pass."""
+    of a conditioning vector.  Variables `<scopes>/GatedResidual[_k]/{entry_scale, entry_offset, exit_scale, exit_offset, res_scale}` and two
+    `<scopes>/fully_connected[_k]/{weights, biases}`, or, with `scope`, all of them below `<scope>/` (a scope given twice shares them); res_scale
+    starts at 0.1.  `save8` ('e4m3' | 'int8'): activations kept in 8 bits for the backward pass."""
     act, foreign = _act_code(activation_fn)
     if foreign is not None:
         raise Exception("gated_res_block takes relu, leaky_relu or no activation")
     C = inputs.shape[-1]
     F = C if num_hidden is None else num_hidden
-    name = scope if scope is not None else _unique("GatedResidual")
-    n1, n2 = _unique("fully_connected"), _unique("fully_connected")
+    if scope is not None:
+        name, n1, n2 = scope, scope + "/fully_connected", scope + "/fully_connected_1"
+    else:
+        name, n1, n2 = _unique("GatedResidual"), _unique("fully_connected"), _unique("fully_connected")
 
     def var(leaf, value):
         return lib.param(name + "/" + leaf, np.full(C, value, dtype="float32"))
