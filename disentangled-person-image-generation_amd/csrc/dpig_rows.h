@@ -138,33 +138,46 @@ __device__ __forceinline__ float inv_sqrt(float a) {
     return f == f ? f : r;                                    // (1 / sqrt of infinity is zero, of zero infinite)
 }
 
+// A row's sum from the sums of its vectors in a lane.  One of 8 lanes x 3 vectors is (S0 + S1) + S2 with S the sums over lanes of one vector each, which is
+// the order in which 32 lanes of one vector add up ((S2 + zeros) there); likewise 16 x 3 and 64 x 1, 64 x 3 and 256 x 1, and 32 x 3 and 64 x 2 with the two
+// vectors apart.  So a row's statistics do not depend on its layout: the exit's norms are the entry's bit for bit whatever either chooses.
+template <int LPR, int NV> constexpr bool vectors_apart() { return NV == 3 || (LPR == 64 && NV == 2); }
+template <int LPR, int NV, int NS> __device__ __forceinline__ float row_sum(float (&s)[NS], float (*red)[4]) {
+    row_sums<LPR, NS>(s, red);
+    float t = s[0];
+#pragma unroll
+    for (int j = 1; j < NS; ++j) t += s[j];
+    return t;
+}
 // Statistics of a row held in registers, and the row normed in place: mean first, then the sum of squares about it (no cancellation).
 // n[j] <= 0: a vector outside the row (zero); what is behind a partial vector's end is ignored and comes out as zero.
 template <int LPR, int NV, bool RAG>
 __device__ __forceinline__ void whiten(float (&v)[NV][8], const int (&n)[NV], float C, float rC, bool layer, float eps, float (*red)[4], float* mean,
                                        float* rstd) {
-    float s[1];
+    constexpr bool APART = vectors_apart<LPR, NV>();
+    constexpr int NS = APART ? NV : 1;
+    float s[NS];
     float mu = 0.f;
     if (layer) {
-        s[0] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NS; ++j) s[j] = 0.f;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[0] += !RAG || e < n[j] ? v[j][e] : 0.f;
-        row_sums<LPR, 1>(s, red);
-        mu = over_count(s[0], C, rC);
+            for (int e = 0; e < 8; ++e) s[APART ? j : 0] += !RAG || e < n[j] ? v[j][e] : 0.f;
+        mu = over_count(row_sum<LPR, NV>(s, red), C, rC);
     }
-    s[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) s[j] = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const bool in = RAG ? e < n[j] : n[j] > 0;
             v[j][e] = in ? v[j][e] - mu : 0.f;
-            s[0] += v[j][e] * v[j][e];
+            s[APART ? j : 0] = fmaf(v[j][e], v[j][e], s[APART ? j : 0]);
         }
-    row_sums<LPR, 1>(s, red);
-    const float r = inv_sqrt(over_count(s[0], C, rC) + eps);
+    const float r = inv_sqrt(over_count(row_sum<LPR, NV>(s, red), C, rC) + eps);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -207,9 +220,7 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
     }
 }
 
-// Launch shape of a row length: lanes per row and vectors per lane.  One or two vectors a lane up to 4096 channels; where that leaves a lane in
-// three or more idle (just above a power of two) and there are rows enough for four sets a CU, a quarter of the lanes with three each: 32768 rows of 640
-// channels, the exit's gradient, 24 us instead of 30.  Where the lanes are better filled it does not pay (384 channels: 41.6 against 39.9 us).
+// Launch shape of a row length: lanes per row and vectors per lane.  One or two vectors a lane up to 4096 channels.
 #define DPIG_ROWS_DISPATCH2(C, CALL)                     \
     do {                                                 \
         if ((C) <= 64) { CALL(8, 1); }                   \
@@ -221,23 +232,30 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
         else if ((C) <= 4096) { CALL(256, 2); }          \
         else { CALL(256, 4); }                           \
     } while (0)
-#define DPIG_ROWS_DISPATCH(C, THREE, CALL)               \
-    do {                                                 \
-        if (!(THREE)) DPIG_ROWS_DISPATCH2(C, CALL);      \
-        else if ((C) <= 160) { CALL(8, 3); }             \
-        else if ((C) <= 320) { CALL(16, 3); }            \
-        else if ((C) <= 640) { CALL(32, 3); }            \
-        else { CALL(64, 3); }                            \
-    } while (0)
 inline int lanes_per_row2(int C) { return C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256; }
+// Between a power of two and one and a half of it (129 .. 192, 257 .. 384, 513 .. 768, 1025 .. 1536 channels) a quarter to a half of those lanes' vectors are
+// idle.  A quarter of the lanes with three vectors each leave fewer idle and ask for more at a time, once there are rows for four sets a CU; what a lane
+// holds of three vectors must be small for that.  Where they are taken, us with two / three:
+//   entry, bf16 whole rows         32768 x 136 9.8 / 8.7, 131072 x 320 48.1 / 36.7, 65536 x 640 40.7 / 36.2, 32768 x 1280 43.7 / 36.1
+//   entry, fp32 with a checkpoint  131072 x 320 90.1 / 81.1, 32768 x 1280 87.8 / 80.5, 16384 x 320 14.1 / 14.1, 32768 x 160 13.4 / 14.2
+//   gradients, bf16                from x 262144 x 136 59.2 / 45.8, 32768 x 1280 68.6 / 48.8, 16384 x 320 17.4 / 17.0, 32768 x 160 16.7 / 17.8
+//   gradients, from a checkpoint   bf16 262144 x 136 53.0 / 41.6, 32768 x 1280 64.7 / 43.9; fp32 131072 x 320 95.4 / 88.0, 16384 x 320 20.8 / 21.9
+//   exits, bf16 whole rows of 513 .. 768 with the next norm or a gate per row: 65536 x 640 98.9 / 79.7 and 135.0 / 127.5, 8192 x 640 21.1 / 19.5 and
+//                                  22.9 / 20.7; with both 193 / 221, with neither 30.8 / 34.9 (32768 rows)
+// Elsewhere two vectors are as fast or faster, three / two: fp32 entry without a checkpoint 0.85 .. 1.08, fp32 gradients from x 0.92 .. 1.25, ragged bf16
+// entry 0.84 .. 1.14, the other exits 0.81 .. 1.97 (two operands and five rows of parameters).
 inline bool three_vectors(int64_t nrows, int C) {
     const int lanes = C > 1024 ? 64 : C > 512 ? 32 : C > 256 ? 16 : 8;
-    const bool thin = (C > 128 && C <= 160) || (C > 256 && C <= 320) || (C > 512 && C <= 640) || (C > 1024 && C <= 1280);
-    return thin && nrows * lanes >= 4L * kNumCU * NT;
+    return C > 16 * lanes && C <= 24 * lanes && nrows * lanes >= 4L * kNumCU * NT;
 }
-inline int lanes_per_row(int64_t nrows, int C) {
-    return !three_vectors(nrows, C) ? lanes_per_row2(C) : C <= 160 ? 8 : C <= 320 ? 16 : C <= 640 ? 32 : 64;
-}
+#define DPIG_ROWS_DISPATCH3(C, CALL)                     \
+    do {                                                 \
+        if ((C) <= 192) { CALL(8, 3); }                  \
+        else if ((C) <= 384) { CALL(16, 3); }            \
+        else if ((C) <= 768) { CALL(32, 3); }            \
+        else { CALL(64, 3); }                            \
+    } while (0)
+inline int lanes_per_row3(int C) { return C <= 192 ? 8 : C <= 384 ? 16 : C <= 768 ? 32 : 64; }
 inline bool vec_ok(const void* p, int64_t ld, int esize) { return aligned16(p) && (ld * esize) % 16 == 0; }
 
 }  // namespace rows

@@ -28,6 +28,7 @@ struct BwdP {
     float* partial;
     long lddy, ldx, ldacc, lddx, nrows, chunk, per, ngroups;     // chunk: rows of a piece / groups of a workgroup
     int C, layer, fmt, ld8, gate_bf16, pieces;
+    bool three;                          // pieces form: three vectors a lane
     float rC;
 };
 
@@ -305,9 +306,13 @@ template <typename T> inline void launch_rows_as(const BwdP& p, bool groups, uns
         if (saved) hipLaunchKernelGGL((rows_bwd_groups_kernel<T, L, N, true>), grid, dim3(NT), 0, st, p);                 \
         else hipLaunchKernelGGL((rows_bwd_groups_kernel<T, L, N, false>), grid, dim3(NT), 0, st, p);                      \
     } while (0)
+#define CALL_SAVED(L, N) do { if (rag) CALL_RS(L, N, true, true); else CALL_RS(L, N, false, true); } while (0)
     if (groups) DPIG_ROWS_DISPATCH2(p.C, CALL_GROUPS);
-    else DPIG_ROWS_DISPATCH(p.C, three_vectors(p.nrows, p.C), CALL);
+    else if (!p.three) DPIG_ROWS_DISPATCH2(p.C, CALL);
+    else if constexpr (sizeof(T) == 2) DPIG_ROWS_DISPATCH3(p.C, CALL);
+    else DPIG_ROWS_DISPATCH3(p.C, CALL_SAVED);
 #undef CALL
+#undef CALL_SAVED
 #undef CALL_GROUPS
 #undef CALL_RS
 }

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(FC * FL) void rows_final_kernel(const FinP p) {
 // Groups shorter than this run in the groups form: a piece of fewer rows would leave more partial sums than it reads.
 constexpr long SHORT_GROUP = 16;
 struct Plan {
-    bool groups;
+    bool groups, three;
     long chunk, pieces, blocks, blocks2;          // blocks2 > 1: workgroups (y) of rows_groups_kernel, whose sums a second launch adds
 };
 // workgroups: one per set of rows taken at a time while that is at most one per CU, then about eight sets each, at most two per CU: more of them
@@ -158,10 +158,12 @@ static long want_blocks(long sets) {
     const long b = sets / 8;
     return b < kNumCU ? kNumCU : (b > 2 * kNumCU ? 2 * kNumCU : b);
 }
-static Plan plan(int64_t nrows, int C, bool gated, int64_t groups) {
+// (three: the tensors' type, or a checkpoint, allows three vectors a lane)
+static Plan plan(int64_t nrows, int C, bool gated, int64_t groups, bool three) {
     Plan q = {};
     const long per = nrows / groups;
-    long rpb = NT / lanes_per_row(nrows, C);
+    q.three = three && three_vectors(nrows, C);
+    long rpb = NT / (q.three ? lanes_per_row3(C) : lanes_per_row2(C));
     auto up = [](long a, long b) { return (a + b - 1) / b; };
     if (gated && groups > 1 && per < SHORT_GROUP) {
         q.groups = true;
@@ -185,6 +187,11 @@ static Plan plan(int64_t nrows, int C, bool gated, int64_t groups) {
 }
 static size_t ws_bytes(const Plan& q, int C) {
     return (size_t)(q.blocks + (!q.groups && q.blocks2 > 1 ? q.blocks2 : 0)) * 2 * C * sizeof(float);
+}
+// what is enough for either layout: the queries know neither the tensors' type nor whether they come from a checkpoint
+static size_t ws_bytes(int64_t nrows, int C, bool gated, int64_t groups) {
+    const size_t a = ws_bytes(plan(nrows, C, gated, groups, false), C), b = ws_bytes(plan(nrows, C, gated, groups, true), C);
+    return a > b ? a : b;
 }
 
 static void launch_sums(FinP f, const Plan& q, int64_t groups, hipStream_t st) {
@@ -229,7 +236,7 @@ using namespace dpig;
 
 extern "C" size_t dpig_rownorm_bwd_workspace_bytes(int64_t nrows, int C) {
     if (nrows <= 0 || C <= 0 || C > rows::C_MAX) return 0;
-    return rows::ws_bytes(rows::plan(nrows, C, false, 1), C);
+    return rows::ws_bytes(nrows, C, false, 1);
 }
 
 extern "C" int dpig_rownorm_bwd(const void* dy, int is_bf16, int64_t lddy, const void* x, int64_t ldx, int fmt, const uint8_t* codes,
@@ -239,14 +246,14 @@ extern "C" int dpig_rownorm_bwd(const void* dy, int is_bf16, int64_t lddy, const
     if (int rc = rows::check_bwd("rownorm_bwd", nrows, C, kind, dy, x, codes, scales, fmt, mean, rstd, dx, lddy, ldx, lddx)) return rc;
     if (accum && ldacc < C) return fail(DPIG_EINVAL, "rownorm_bwd: row stride below the channel count");
     const bool params = dscale || doffset;
-    const rows::Plan q = rows::plan(nrows, C, false, 1);
+    const rows::Plan q = rows::plan(nrows, C, false, 1, is_bf16 || codes);
     if (params && (!ws || ws_bytes < rows::ws_bytes(q, C))) return fail(DPIG_ENOMEM, "rownorm_bwd: workspace too small");
     hipStream_t st = static_cast<hipStream_t>(stream);
     rows::BwdP p = {};
     p.dy = dy; p.x = x; p.accum = accum; p.dx = dx; p.codes = codes; p.scales = scales; p.mean = mean; p.rstd = rstd; p.scale = scale;
     p.partial = params ? static_cast<float*>(ws) : nullptr;
     p.lddy = lddy; p.ldx = ldx; p.ldacc = ldacc; p.lddx = lddx; p.nrows = nrows; p.chunk = q.chunk; p.per = nrows; p.ngroups = 1;
-    p.C = C; p.layer = kind == DPIG_NORM_LAYER; p.fmt = fmt; p.ld8 = act8::padded(C); p.pieces = (int)q.pieces; p.rC = 1.0f / (float)C;
+    p.C = C; p.layer = kind == DPIG_NORM_LAYER; p.fmt = fmt; p.ld8 = act8::padded(C); p.pieces = (int)q.pieces; p.three = q.three; p.rC = 1.0f / (float)C;
     if (is_bf16) rows::launch_rows<rows::bf16_t>(p, q.groups, (unsigned)q.blocks, st);
     else rows::launch_rows<float>(p, q.groups, (unsigned)q.blocks, st);
     if (params) {
@@ -259,7 +266,7 @@ extern "C" int dpig_rownorm_bwd(const void* dy, int is_bf16, int64_t lddy, const
 
 extern "C" size_t dpig_gated_residual_bwd_workspace_bytes(int64_t nrows, int C, int64_t groups) {
     if (nrows <= 0 || C <= 0 || C > rows::C_MAX || groups < 0 || (groups > 0 && nrows % groups != 0)) return 0;
-    return rows::ws_bytes(rows::plan(nrows, C, groups > 0, groups > 0 ? groups : 1), C);
+    return rows::ws_bytes(nrows, C, groups > 0, groups > 0 ? groups : 1);
 }
 
 extern "C" int dpig_gated_residual_bwd(const void* dout, int is_bf16, int64_t lddo, const void* f, int64_t ldf, int fmt, const uint8_t* codes,
@@ -272,7 +279,7 @@ extern "C" int dpig_gated_residual_bwd(const void* dout, int is_bf16, int64_t ld
     if (dgate && !gate) return fail(DPIG_EINVAL, "gated_residual_bwd: a gate gradient without a gate");
     if (!gate) groups = 1;
     const bool sums = dscale || doffset || dres_scale, params = sums || dgate;
-    const rows::Plan q = rows::plan(nrows, C, gate != nullptr, groups);
+    const rows::Plan q = rows::plan(nrows, C, gate != nullptr, groups, is_bf16 || codes);
     if (q.blocks > 0x7fffffffL) return fail(DPIG_EINVAL, "gated_residual_bwd: too many gate groups");
     if (params && (!ws || ws_bytes < rows::ws_bytes(q, C))) return fail(DPIG_ENOMEM, "gated_residual_bwd: workspace too small");
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -282,6 +289,7 @@ extern "C" int dpig_gated_residual_bwd(const void* dout, int is_bf16, int64_t ld
     p.partial = (q.groups ? sums : params) ? static_cast<float*>(ws) : nullptr;
     p.lddy = lddo; p.ldx = ldf; p.lddx = lddf; p.nrows = nrows; p.chunk = q.chunk; p.per = nrows / groups; p.ngroups = groups;
     p.C = C; p.layer = kind == DPIG_NORM_LAYER; p.fmt = fmt; p.ld8 = act8::padded(C); p.gate_bf16 = gate_bf16; p.pieces = (int)q.pieces;
+    p.three = q.three;
     p.rC = 1.0f / (float)C;
     if (is_bf16) rows::launch_rows<rows::bf16_t>(p, q.groups, (unsigned)q.blocks, st);
     else rows::launch_rows<float>(p, q.groups, (unsigned)q.blocks, st);

@@ -192,6 +192,24 @@ __global__ __launch_bounds__(NT) void exit_fwd_kernel(const ExitP p) {
     }
 }
 
+// rows per workgroup: a multiple of the rows it takes at a time, at most `per_cu` workgroups per CU
+inline long fwd_chunk(int64_t nrows, int lanes, long per_cu) {
+    const long rpb = NT / lanes;
+    const long want = per_cu * kNumCU;
+    long it = (nrows + rpb * want - 1) / (rpb * want);
+    return (it < 1 ? 1 : it) * rpb;
+}
+// The entry's registers let eight workgroups share a CU, the exit's four.  More of them than fit come in rounds: that evens out HBM where there is much
+// to move (32768 x 256 fp32 with the next norm, 134 MB: 25.0 us in two rounds, 27.0 in one) but costs each round's start where there is little
+// (4096 x 2048 bf16 with the next norm, 67 MB: 16.4 / 14.7; 8192 x 512: 11.0 / 9.6), and a last round that is not full costs as much as a full one
+// (9001 x 333 fp32: 1.1 rounds 17.0, one 13.2; 60001 x 333: 1.8 rounds 74, one 71).
+constexpr long ENTRY_PER_CU = 8, EXIT_PER_CU = 4, EXIT_ONE_ROUND_BYTES = 96L << 20;
+inline long exit_chunk(int64_t nrows, int lanes, long bytes) {
+    const long one = fwd_chunk(nrows, lanes, EXIT_PER_CU), two = fwd_chunk(nrows, lanes, 2 * EXIT_PER_CU);
+    const long groups = (nrows + two - 1) / two, rounds = (groups + EXIT_PER_CU * kNumCU - 1) / (EXIT_PER_CU * kNumCU);
+    return bytes < EXIT_ONE_ROUND_BYTES || one < rounds * two ? one : two;
+}
+
 // the kernels on tensors of type T; each type is compiled in a file of its own
 template <typename T> int entry_fwd(EntryP p, hipStream_t st);
 template <typename T> int exit_fwd(ExitP p, hipStream_t st);
@@ -199,6 +217,8 @@ template <typename T> int exit_fwd(ExitP p, hipStream_t st);
 template <typename T> inline int entry_fwd_as(EntryP p, hipStream_t st) {
     const bool rag = p.C % 8 != 0 || !vec_ok(p.x, p.ldx, sizeof(T)) || !vec_ok(p.y, p.ldy, sizeof(T));
     const bool save = p.save.codes != nullptr;
+    const bool three = (sizeof(T) == 2 ? !rag : save) && three_vectors(p.nrows, p.C);
+    p.chunk = fwd_chunk(p.nrows, three ? lanes_per_row3(p.C) : lanes_per_row2(p.C), ENTRY_PER_CU);
     const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
 #define CALL_RS(L, N, R, S) hipLaunchKernelGGL((entry_fwd_kernel<T, L, N, R, S>), grid, dim3(NT), 0, st, p)
 #define CALL(L, N)                                                                                                         \
@@ -206,8 +226,14 @@ template <typename T> inline int entry_fwd_as(EntryP p, hipStream_t st) {
         if (rag) { if (save) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
         else { if (save) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
     } while (0)
-    DPIG_ROWS_DISPATCH(p.C, three_vectors(p.nrows, p.C), CALL);
+#define CALL_WHOLE(L, N) do { if (save) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); } while (0)
+#define CALL_SAVE(L, N) do { if (rag) CALL_RS(L, N, true, true); else CALL_RS(L, N, false, true); } while (0)
+    if (!three) DPIG_ROWS_DISPATCH2(p.C, CALL);
+    else if constexpr (sizeof(T) == 2) DPIG_ROWS_DISPATCH3(p.C, CALL_WHOLE);
+    else DPIG_ROWS_DISPATCH3(p.C, CALL_SAVE);
 #undef CALL
+#undef CALL_WHOLE
+#undef CALL_SAVE
 #undef CALL_RS
     return check_launch("rownorm_fwd");
 }
@@ -215,9 +241,10 @@ template <typename T> inline int exit_fwd_as(ExitP p, hipStream_t st) {
     const int z = sizeof(T);
     const bool rag = p.C % 8 != 0 || !vec_ok(p.x, p.ldx, z) || !vec_ok(p.f, p.ldf, z) || !vec_ok(p.out, p.ldo, z) ||
                      (p.h != nullptr && !vec_ok(p.h, p.ldh, z));
-    const bool next = p.h != nullptr;
+    const bool next = p.h != nullptr, each = p.gate != nullptr && p.per == 1;
+    const bool three = sizeof(T) == 2 && !rag && next != each && p.C > 512 && p.C <= 768 && three_vectors(p.nrows, p.C);
+    p.chunk = exit_chunk(p.nrows, three ? lanes_per_row3(p.C) : lanes_per_row2(p.C), (long)p.nrows * p.C * z * (next ? 4 : 3));
     const dim3 grid((unsigned)((p.nrows + p.chunk - 1) / p.chunk));
-    const bool each = p.gate != nullptr && p.per == 1;
 #define CALL_E(L, N, R, S, E) hipLaunchKernelGGL((exit_fwd_kernel<T, L, N, R, S, E>), grid, dim3(NT), 0, st, p)
 #define CALL_RS(L, N, R, S) do { if (each) CALL_E(L, N, R, S, true); else CALL_E(L, N, R, S, false); } while (0)
 #define CALL(L, N)                                                                                                         \
@@ -225,7 +252,10 @@ template <typename T> inline int exit_fwd_as(ExitP p, hipStream_t st) {
         if (rag) { if (next) CALL_RS(L, N, true, true); else CALL_RS(L, N, true, false); }                                 \
         else { if (next) CALL_RS(L, N, false, true); else CALL_RS(L, N, false, false); }                                   \
     } while (0)
-    DPIG_ROWS_DISPATCH(p.C, three_vectors(p.nrows, p.C), CALL);
+    if (!three) DPIG_ROWS_DISPATCH2(p.C, CALL);
+    else if constexpr (sizeof(T) == 2) {
+        if (next) CALL_E(32, 3, false, true, false); else CALL_E(32, 3, false, false, true);
+    }
 #undef CALL
 #undef CALL_E
 #undef CALL_RS

@@ -10,24 +10,6 @@ namespace rows {
 template <> int entry_fwd<bf16_t>(EntryP p, hipStream_t st);      // dpig_rows_fwd_bf16.hip
 template <> int exit_fwd<bf16_t>(ExitP p, hipStream_t st);
 
-// rows per workgroup: a multiple of the rows it takes at a time, at most `per_cu` workgroups per CU
-static long fwd_chunk(int64_t nrows, int C, long per_cu) {
-    const long rpb = NT / lanes_per_row(nrows, C);
-    const long want = per_cu * kNumCU;
-    long it = (nrows + rpb * want - 1) / (rpb * want);
-    return (it < 1 ? 1 : it) * rpb;
-}
-// The entry's registers let eight workgroups share a CU, the exit's four.  More of them than fit come in rounds: that evens out HBM where there is much
-// to move (32768 x 256 fp32 with the next norm, 134 MB: 25.0 us in two rounds, 27.0 in one) but costs each round's start where there is little
-// (4096 x 2048 bf16 with the next norm, 67 MB: 16.4 / 14.7; 8192 x 512: 11.0 / 9.6), and a last round that is not full costs as much as a full one
-// (9001 x 333 fp32: 1.1 rounds 17.0, one 13.2; 60001 x 333: 1.8 rounds 74, one 71).
-constexpr long ENTRY_PER_CU = 8, EXIT_PER_CU = 4, EXIT_ONE_ROUND_BYTES = 96L << 20;
-static long exit_chunk(int64_t nrows, int C, long bytes) {
-    const long one = fwd_chunk(nrows, C, EXIT_PER_CU), two = fwd_chunk(nrows, C, 2 * EXIT_PER_CU);
-    const long groups = (nrows + two - 1) / two, rounds = (groups + EXIT_PER_CU * kNumCU - 1) / (EXIT_PER_CU * kNumCU);
-    return bytes < EXIT_ONE_ROUND_BYTES || one < rounds * two ? one : two;
-}
-
 static int check_rows(const char* who, int64_t nrows, int C, int kind) {
     if (nrows <= 0 || nrows > (1L << 40)) return fail(DPIG_EINVAL, "%s: bad row count", who);
     if (C <= 0 || C > C_MAX) return fail(DPIG_EINVAL, "%s: channels must be 1 .. %d", who, C_MAX);
@@ -54,8 +36,8 @@ extern "C" int dpig_rownorm_fwd(const void* x, int is_bf16, int64_t ldx, int64_t
     if (int rc = rows::check_save("rownorm_fwd", fmt, codes, scales)) return rc;
     if (!x || !y || !rstd || (kind == DPIG_NORM_LAYER && !mean)) return fail(DPIG_EINVAL, "rownorm_fwd: null pointer");
     if (ldx < C || ldy < C) return fail(DPIG_EINVAL, "rownorm_fwd: row stride below the channel count");
-    rows::EntryP p = {x, y, scale, offset, kind == DPIG_NORM_LAYER ? mean : nullptr, rstd, (long)ldx, (long)ldy, (long)nrows,
-                      rows::fwd_chunk(nrows, C, rows::ENTRY_PER_CU), C, kind == DPIG_NORM_LAYER, eps, 1.0f / (float)C, {codes, scales, fmt, act8::padded(C)}};
+    rows::EntryP p = {x, y, scale, offset, kind == DPIG_NORM_LAYER ? mean : nullptr, rstd, (long)ldx, (long)ldy, (long)nrows, 0, C,
+                      kind == DPIG_NORM_LAYER, eps, 1.0f / (float)C, {codes, scales, fmt, act8::padded(C)}};
     hipStream_t st = static_cast<hipStream_t>(stream);
     return is_bf16 ? rows::entry_fwd<rows::bf16_t>(p, st) : rows::entry_fwd<float>(p, st);
 }
@@ -78,8 +60,7 @@ extern "C" int dpig_gated_residual_fwd(const void* x, int64_t ldx, const void* f
     }
     const int ld8 = act8::padded(C);
     rows::ExitP p = {x, f, out, h, scale, offset, res_scale, scale2, offset2, gate, kind == DPIG_NORM_LAYER ? mean : nullptr, rstd,
-                     kind2 == DPIG_NORM_LAYER ? mean2 : nullptr, rstd2, (long)ldx, (long)ldf, (long)ldo, (long)ldh, (long)nrows,
-                     rows::exit_chunk(nrows, C, (long)nrows * C * (is_bf16 ? 2 : 4) * (h ? 4 : 3)), gate ? (long)(nrows / groups) : (long)nrows, C, kind == DPIG_NORM_LAYER,
+                     kind2 == DPIG_NORM_LAYER ? mean2 : nullptr, rstd2, (long)ldx, (long)ldf, (long)ldo, (long)ldh, (long)nrows, 0, gate ? (long)(nrows / groups) : (long)nrows, C, kind == DPIG_NORM_LAYER,
                      kind2 == DPIG_NORM_LAYER, gate_bf16, eps, eps2, 1.0f / (float)C, {codes, scales, fmt, ld8},
                      {h ? codes2 : nullptr, scales2, fmt2, ld8}};
     hipStream_t st = static_cast<hipStream_t>(stream);

@@ -61,3 +61,26 @@ def test_exit_gradient_from_checkpoints_of_groups(dev, rows, C, groups, dtype, f
     T._close(dr, (d * G * n).sum(0), R.sums_error(d * G * nmag, rows))
     t, tm = ((d * res.double() * k).reshape(groups, per, C) for k in (n, nmag))
     T._close(dg, t.sum(1), torch.stack([R.sums_error(q, per) for q in tm]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,C", WHOLE + RAGGED)
+def test_a_rows_result_does_not_depend_on_the_layout(dev, rows, C, dtype):
+    """The last rows of a large call are, bit for bit, what a small call on them gives: entry with and without a checkpoint, exits with and without the next
+    norm, gates per row and per group."""
+    H = T._H()
+    x, f = T._rand(rows, C, 1, dtype).to(dev), T._rand(rows, C, 2, dtype).to(dev)
+    s, o, r = (T._vec(C, i).to(dev) for i in (1, 2, 3))
+    gate = T._rand(rows, C, 4, dtype).to(dev)
+    n = 50
+    xt, ft, gt = (t[-n:].contiguous() for t in (x, f, gate))
+    for save in (None, "e4m3"):
+        y, mean, rstd, a = H.rownorm_fwd(x, s, o, T.EPS, "layer", save8=save)
+        yt, mt, rt, at = H.rownorm_fwd(xt, s, o, T.EPS, "layer", save8=save)
+        assert torch.equal(y[-n:], yt) and torch.equal(mean[-n:], mt) and torch.equal(rstd[-n:], rt)
+        assert save is None or (torch.equal(a.codes[-n:], at.codes) and torch.equal(a.scales[-n:], at.scales))
+    for nxt in (None, (s, o, T.EPS, "rms")):
+        for g, t in ((gate, gt), (None, None), (gate[0], gate[0])):
+            p, q = H.gated_residual_fwd(x, f, s, o, g, r, T.EPS, "layer", next_norm=nxt), H.gated_residual_fwd(xt, ft, s, o, t, r, T.EPS, "layer", next_norm=nxt)
+            assert torch.equal(p[0][-n:], q[0]) and torch.equal(p[1][-n:], q[1]) and torch.equal(p[2][-n:], q[2])
+            assert nxt is None or (torch.equal(p[4][0][-n:], q[4][0]) and torch.equal(p[4][2][-n:], q[4][2]))
