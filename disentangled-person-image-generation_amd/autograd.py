@@ -326,7 +326,8 @@ def _sink_small(p, g):
 # The 16-image 128 x 64 training step holds 1.60 GB beyond its parameters instead of 3.33 in 'f32w', 39.3 ms instead of 37.8, and 1.24 GB instead
 # of 1.68 in 'bf16', 16.4 ms instead of 14.3 (both uncaptured).
 # The backward pass reads them: activation masks and the filter gradients of 1x1 / fully connected layers directly, other filter gradients from
-# values decoded into a scratch tensor.  Forward results are unchanged; filter gradients see inputs rounded to 8 bits.
+# values decoded into a scratch tensor.  Forward results are unchanged, and so are input gradients where the activations are finite (an infinity or a NaN in
+# one masks the 32 channels of its group, and gives NaN in the filter gradient that reads it); filter gradients see inputs rounded to 8 bits.
 SAVE8 = [None]
 
 

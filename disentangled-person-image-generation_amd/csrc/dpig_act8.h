@@ -12,7 +12,8 @@
 //     checkpoint of a ReLU / LeakyReLU output then has the sign pattern of the output and serves as the activation's mask.  It costs
 //     at most one smallest code of error there (2^-9 s, 1 s) instead of half of one;
 //   * a group that holds a NaN or an infinity gets the scale byte 255 and zero codes: it comes back as NaN throughout, so an overflow
-//     of the forward pass is seen in the gradients, and no value has to be tested when it is read;
+//     of the forward pass is seen where values are read (filter gradients, norms' gradients), and none has to be tested then.  A mask is
+//     read from the codes alone: the whole group counts as not positive, its finite neighbours of an infinity included;
 //   * e is kept within [-116, 119] (E4M3) / [-116, 121] (INT8): every decoded value is a normal, finite fp32 / bf16 number.  What is larger than
 //     the last scale's largest code (1.75 * 2^127) is stored as that code.
 #pragma once

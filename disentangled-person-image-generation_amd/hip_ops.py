@@ -1558,7 +1558,8 @@ def act8_load(a, dtype=F32):
 
 
 def act8_act_bwd(dy, a, act, alpha=0.2):
-    """dz = dy * act'(y), y the ReLU / LeakyReLU output that the checkpoint `a` holds (its codes keep y's sign)."""
+    """dz = dy * act'(y), y the ReLU / LeakyReLU output that the checkpoint `a` holds (its codes keep y's sign; a group that held a value that was
+    not finite counts as not positive: dy times 0 or alpha for all of its 32 channels)."""
     if act not in (ACT_RELU, ACT_LRELU):
         raise RuntimeError("act8_act_bwd: the activation must be ReLU or LeakyReLU")
     dy, rows, C, ld = _rows_of(dy, "dy")

@@ -635,7 +635,8 @@ int dpig_act8_store(const void* x, int is_bf16, int64_t ldx, int64_t rows, int C
                     void* stream);
 int dpig_act8_load(const uint8_t* codes, const uint8_t* scales, int64_t rows, int C, int fmt, void* y, int is_bf16, int64_t ldy,
                    void* stream);
-/* dz = dy * act'(y) with the sign of y read from its checkpoint (ReLU, LeakyReLU). */
+/* dz = dy * act'(y) with the sign of y read from its checkpoint (ReLU, LeakyReLU).  The scales are not read: a group that was not finite (zero codes)
+ * counts as not positive. */
 int dpig_act8_act_bwd(const void* dy, int is_bf16, int64_t lddy, const uint8_t* codes, int64_t rows, int C, int fmt, int act, float alpha,
                       void* dz, int64_t lddz, void* stream);
 

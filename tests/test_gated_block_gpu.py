@@ -360,3 +360,34 @@ def test_layers_wider_than_a_checkpoints_product(dev):
         assert np.isfinite(float(o["d_loss"])) and bool(torch.isfinite(tr.G_flat.flat).all())
     assert first[0] == first[1]
     lib.delete_all_params(); slim.reset_scopes()
+
+
+@pytest.mark.parametrize("act,off", [(1, 0.0), (2, 0.2)])
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_activations_that_are_not_finite_under_checkpoints(dev, fmt, act, off):
+    """As documented: the 32 channels that share a scale with an infinity count as not positive in the activation's mask, every other gradient keeps its
+    bits, and the filter gradient of the layer that reads the infinity is NaN in that group's rows."""
+    A, H = _mods()
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(12, 64, generator=g).to(dev)
+    w, w2 = (torch.randn(*n, generator=g).to(dev) for n in ((64, 96), (96, 40)))
+    x[5] = 3e38
+    w[:, 70] = 3.0                                                       # y[5, 70] overflows
+    w[:, :70], w[:, 71:] = w[:, :70] * 1e-39, w[:, 71:] * 1e-39          # ... and nothing else of the row
+    got = []
+    for save8 in (None, fmt):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, w2)]
+        y = A.linear(leaves[0], leaves[1], act=act, save8=save8)
+        assert torch.isinf(y).nonzero().tolist() == [[5, 70]]
+        A.linear(y, leaves[2], save8=save8).backward(torch.ones(12, 40, device=dev))
+        got.append([t.grad for t in leaves] + [y.detach()])
+    (dx0, _, _, y0), (dx1, dw1, dw2, y1) = got
+    assert torch.equal(y0, y1)
+    keep = [r for r in range(12) if r != 5]
+    assert torch.equal(dx0[keep], dx1[keep])
+    dy = w2.sum(1)
+    m = torch.where(y0[5] > 0, torch.ones(96, device=dev), torch.full((96,), off, device=dev))
+    m[64:] = off                                                         # the group of channel 70
+    want = (dy.double() * m.double()) @ w.double().t().contiguous()
+    assert float((dx1[5].double() - want).abs().max()) <= R.U * 200 * float((dy.double().abs() * m.double()) @ w.double().abs().t().contiguous().amax(1))
+    assert torch.isnan(dw2).all(1).nonzero().flatten().tolist() == list(range(64, 96)) and not bool(torch.isnan(dw2[:64]).any())
