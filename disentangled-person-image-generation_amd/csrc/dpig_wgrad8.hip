@@ -436,15 +436,17 @@ struct Plan { Shape shape; int mtiles, ntiles, nsplit, rows_per_split; };
 static Plan plan(int64_t nrows, int C, int K, bool f32, long row_bytes) {
     Plan q;
     auto up = [](long a, long b) { return (a + b - 1) / b; };
-    // Larger tiles read and decode less per product but leave fewer, larger pieces of work and more partial sums: 256 x 128 pays from about
-    // 10^10 products on (rows x 512 x 512 bf16, both ways: 32768 rows 33.9 / 35.0 us, 65536 rows 59.0 / 53.0; a third of that for fp32 dy: 8192 rows
-    // 28.2 / 27.8, 16384 rows 38.5 / 37.2), 256 x 256 above 2^35 (131072 rows 89.5 / 90.4 us, 262144 rows 175 / 163), unless it is padding that grows.
+    // Larger tiles read and decode less per product but leave fewer, larger pieces of work and more partial sums.  us with the smaller / larger tile:
+    // 256 x 128 pays from about 10^10 products on (bf16 rows x 512 x 512, 24576 rows 29.0 / 30.7, 32768 36.5 / 36.2, 49152 47.3 / 44.5; x 256 x 512, 65536 rows
+    // 39.5 / 40.3, 98304 52.4 / 50.8; a third of that for fp32 dy: rows x 512 x 512, 12288 rows 31.2 / 31.6, 16384 rows 37.5 / 36.9), 256 x 256 from 2^36
+    // (512 x 512, 131072 rows 95.0 / 98.5, 196608 133 / 131, 262144 171 / 170; 768 x 768, 98304 rows 138 / 142, 131072 186 / 180), unless it is padding
+    // that grows.
     const double products = (double)nrows * C * K * (f32 ? 3 : 1);
     auto area = [&](Shape t) { return up(C, t.tm) * t.tm * up(K, t.tn) * t.tn; };
     q.shape = f32 ? SMALL32 : SMALL;
     const Shape wide = f32 ? WIDE32 : WIDE;
     if (products > 0x1.4p33 && area(wide) <= area(q.shape) * 5 / 4) q.shape = wide;
-    if (!f32 && products > 0x1p35 && area(LARGE) <= area(q.shape) * 9 / 8) q.shape = LARGE;
+    if (!f32 && products >= 0x1p36 && area(LARGE) <= area(q.shape) * 9 / 8) q.shape = LARGE;
     q.mtiles = (int)up(C, q.shape.tm);
     q.ntiles = (int)up(K, q.shape.tn);
     const long tiles = (long)q.mtiles * q.ntiles, rt = up(nrows, q.shape.tr);

@@ -188,7 +188,7 @@ def test_linear_wgrad8_reads_every_value_exactly(dev, rows, C, dtype, fmt):
     assert torch.equal(db.cpu(), torch.ones(rows))
 
 
-# the 256 x 128 and 256 x 256 tiles are taken above 10^10 and 2^35 products (fp32 dy: a third of that)
+# the 256 x 128 tile is taken above 10^10 products (fp32 dy: a third of that)
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("rows,C,K,dtype", [(90001, 250, 520, BF16), (90001, 250, 519, BF16), (140001, 500, 520, BF16), (140001, 512, 513, BF16),
                                               (80001, 200, 260, F32)])
@@ -283,3 +283,10 @@ def test_linear_wgrad8_of_rows_far_apart(dev, dtype):
     wide.copy_(dy)
     dw, db = H.linear_wgrad8(H.act8_store(q, "int8"), wide, want_bias=True)
     assert torch.equal(dw.double(), q.double().t().contiguous() @ dy.double()) and torch.equal(db.double(), dy.double().sum(0))
+
+
+# the 256 x 256 tile is taken from 2^36 products on where it pads no more than 9 / 8 of what 256 x 128 does (the shapes above do)
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("rows,C,K", [(270000, 510, 512), (270001, 512, 511), (270017, 250, 1021), (120031, 760, 766)])
+def test_linear_wgrad8_largest_tiles_are_exact_on_integers(dev, rows, C, K, fmt):
+    test_linear_wgrad8_large_tiles_are_exact_on_integers(dev, rows, C, K, BF16, fmt)
