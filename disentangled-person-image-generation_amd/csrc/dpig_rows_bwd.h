@@ -9,9 +9,10 @@
 //   groups   a row's lanes take WHOLE groups (short ones: down to a row each), write dgate themselves and keep gate-weighted sums:
 //            partial [workgroup][2][C]
 // The partials are added in a fixed order by one or two small launches: no atomics, the same bits every time.
-// Bound by HBM (2 to 4 row tensors in and out).  Measured, row pass + sums: 32768 x 384 fp32 with accum 39.0 + 4.2 us (201 MB, 5.2 TB/s in the pass);
-// 131072 x 256 bf16 with accum 52.0 + 4.3; 47915 x 250 bf16 from an int8 checkpoint 16.7 + 4.4; exit 32768 x 640 bf16 from its e4m3 checkpoint, a
-// gate per 4096 rows, 25.2 + 5.6 (105 MB, 4.2 TB/s); 32768 x 512 bf16 with a gate per row 44.7 + 4.8; 8192 x 2048 bf16 29.9 + 5.2.
+// Bound by HBM (2 to 4 row tensors in and out).  Measured (averages under the profiler), row pass + sums: 32768 x 384 fp32 with accum 39.0 + 4.5 us (201 MB,
+// 5.2 TB/s in the pass); 131072 x 256 bf16 with accum 52.2 + 4.8; 47915 x 250 bf16 from an int8 checkpoint 17.0 .. 17.9 + 4; exit, a gate per eighth of
+// the rows: 32768 x 640 bf16 from its e4m3 checkpoint 24.0 + 5.2 (105 MB, 4.4 TB/s), from f 27.1 + 5.2 (126 MB, 4.6 TB/s), 8192 x 2048 bf16 from f
+// 22.2 + 6.2; 32768 x 512 bf16 with a gate per row 43.3 + 4.9.
 #pragma once
 #include "dpig_rows.h"
 

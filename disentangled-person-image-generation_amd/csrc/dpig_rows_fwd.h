@@ -6,9 +6,10 @@
 // Bound by HBM: every operand is read once and every result written once, one wave (or less, or a workgroup) per row with the row in
 // registers; a lane asks for the next row before it works on the present one.  A workgroup takes a contiguous range of rows, so the
 // per-channel operands stay in registers and a gate row is loaded when its group begins.
-// Measured: entry 131072 x 256 bf16 with its e4m3 checkpoint 30.5 us (168 MB, 5.5 TB/s); exit with the next norm 131072 x 128 bf16, a gate per
-// 8192 rows, 27.4 us (134 MB, 4.9 TB/s), 131072 x 640 145 us (4.6 TB/s); exit 9001 x 333 fp32 with a gate per row 13.2 us (48 MB, 3.6 TB/s: three rows
-// a wave, whose ends share lines; 60001 rows 70.5 us, 4.5 TB/s); 64 x 512 fp32 2.9 us, the latency of one load, two sums and one store.
+// Measured (averages under the profiler): entry 131072 x 256 bf16 with its e4m3 checkpoint 30 .. 32 us (168 MB, 5.4 TB/s); exit with the next norm
+// 131072 x 128 bf16, a gate per 8192 rows, 28.5 us (134 MB, 4.7 TB/s), 131072 x 640 152 us (4.4 TB/s); exit 9001 x 333 fp32 with a gate per row 13.3 us
+// (48 MB, 3.6 TB/s: three rows a wave, whose ends share lines; 60001 rows 66 us, 4.8 TB/s); 64 x 512 fp32 3.2 us, the latency of one load, two sums
+// and one store.
 #pragma once
 #include "dpig_rows.h"
 

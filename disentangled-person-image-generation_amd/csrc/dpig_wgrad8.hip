@@ -12,9 +12,10 @@
 // way into LDS) and read with the transposing LDS read.  The rows are split over workgroups until the chip is full; partial sums are
 // joined by a second launch in a fixed order.
 //
-// Measured, product + join: bf16 dy 131072 x 512 x 512 79.4 + 6.6 us (68.7 GFLOP: 865 TFLOP/s in the product; a library product of two bf16
-// operands of that shape takes 361 us), 131072 x 768 x 768 169 us in all (915 TFLOP/s), 32768 x 512 x 512 34, 2048 x 512 x 512 14.7; fp32 dy
-// 131072 x 128 x 128 21.9 + 6.1, 32768 x 512 x 512 47.3 + 6.6 (363 TFLOP/s of fp32 products), 20011 x 250 x 390 22.4 + 5.7.
+// Measured (averages under the profiler), product + join: bf16 dy 131072 x 512 x 512 80 .. 94 + 7.8 us, as the chip holds its clock over a run of them
+// (68.7 GFLOP: 730 .. 860 TFLOP/s in the product; a library product of two bf16 operands of that shape takes 361 us), 131072 x 768 x 768 168 + 12.2 (920
+// TFLOP/s), 32768 x 512 x 512 30.8 + 4.5, 2048 x 512 x 512 11.4 + 4.0, 64 x 512 x 512 5.7 and no join; fp32 dy 131072 x 128 x 128 22.4 + 5.8, 32768 x 512 x 512
+// 48.9 + 6.8 (351 TFLOP/s of fp32 products), 20011 x 250 x 390 25.2 .. 27.5 + 5.8, 64 x 512 x 512 6.2.
 // Of the large product the matrix instructions and barriers alone take 54 us, without the loads it is 69, without decoding and staging 63: the
 // matrix pipe, the LDS port and the loads' waits overlap, but not fully.  Asking L2 for tiles ahead of the loads, or for three and six tiles ahead
 // instead of two, changed nothing.  (The steps of the loop as one expression, one exit behind each: 79.4 us; with a branch of its own each, 82.3.)
