@@ -234,15 +234,15 @@ __device__ __forceinline__ void save8(const Save& q, long r, int lane, const flo
     } while (0)
 inline int lanes_per_row2(int C) { return C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 1024 ? 64 : 256; }
 // Between a power of two and one and a half of it (129 .. 192, 257 .. 384, 513 .. 768, 1025 .. 1536 channels) a quarter to a half of those lanes' vectors are
-// idle.  A quarter of the lanes with three vectors each leave fewer idle and ask for more at a time, once there are rows for four sets a CU; what a lane
-// holds of three vectors must be small for that.  Where they are taken, us with two / three:
+// idle.  A quarter of the lanes (half of them at 513 .. 768) with three vectors each leave fewer idle and ask for more at a time, once there are rows for four
+// sets a CU; what a lane holds of three vectors must be small for that.  Where they are taken, us with one or two / three:
 //   entry, bf16 whole rows         32768 x 136 9.8 / 8.7, 131072 x 320 48.1 / 36.7, 65536 x 640 40.7 / 36.2, 32768 x 1280 43.7 / 36.1
 //   entry, fp32 with a checkpoint  131072 x 320 90.1 / 81.1, 32768 x 1280 87.8 / 80.5, 16384 x 320 14.1 / 14.1, 32768 x 160 13.4 / 14.2
 //   gradients, bf16                from x 262144 x 136 59.2 / 45.8, 32768 x 1280 68.6 / 48.8, 16384 x 320 17.4 / 17.0, 32768 x 160 16.7 / 17.8
 //   gradients, from a checkpoint   bf16 262144 x 136 53.0 / 41.6, 32768 x 1280 64.7 / 43.9; fp32 131072 x 320 95.4 / 88.0, 16384 x 320 20.8 / 21.9
 //   exits, bf16 whole rows of 513 .. 768 with the next norm or a gate per row: 65536 x 640 98.9 / 79.7 and 135.0 / 127.5, 8192 x 640 21.1 / 19.5 and
 //                                  22.9 / 20.7; with both 193 / 221, with neither 30.8 / 34.9 (32768 rows)
-// Elsewhere two vectors are as fast or faster, three / two: fp32 entry without a checkpoint 0.85 .. 1.08, fp32 gradients from x 0.92 .. 1.25, ragged bf16
+// Elsewhere one or two vectors are as fast or faster, three over that: fp32 entry without a checkpoint 0.85 .. 1.08, fp32 gradients from x 0.92 .. 1.25, ragged bf16
 // entry 0.84 .. 1.14, the other exits 0.81 .. 1.97 (two operands and five rows of parameters).
 inline bool three_vectors(int64_t nrows, int C) {
     const int lanes = C > 1024 ? 64 : C > 512 ? 32 : C > 256 ? 16 : 8;
